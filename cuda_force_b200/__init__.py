@@ -11,6 +11,7 @@ from cuda_force_b200.ops import (
     backend_report,
     dequantize_int8,
     fused_residual_rmsnorm,
+    gated_residual_rmsnorm,
     kernel_supports,
     lora_linear,
     lora_linear_int8,
@@ -35,6 +36,7 @@ __all__ = [
     "backend_report",
     "dequantize_int8",
     "fused_residual_rmsnorm",
+    "gated_residual_rmsnorm",
     "kernel_supports",
     "lora_linear",
     "lora_linear_int8",

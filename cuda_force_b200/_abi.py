@@ -85,6 +85,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _p, ctypes.c_float, _p, _p, _p, _int, _p, _int, _p, _p, _i64, _i64, _i64, _i64,
          ctypes.c_float, _int, _p, ctypes.c_size_t, _p],
     ),
+    "cf_gated_residual_rmsnorm": (
+        _int,
+        [_p, _p, _p, _p, _p, _i64, _int, _p, _p, _p, _i64, _i64, ctypes.c_float, ctypes.c_float,
+         _int, _p],
+    ),
+    "cf_gated_residual_rmsnorm_backward_workspace_bytes": (
+        ctypes.c_size_t, [_i64, _i64, _int, _i64]),
+    "cf_gated_residual_rmsnorm_backward": (
+        _int,
+        [_p, _p, _p, _p, _p, _p, _p, _i64, _int, _p, _p, _p, _p, _p, _p, _i64, _i64,
+         ctypes.c_float, _int, _p, ctypes.c_size_t, _p],
+    ),
     "cf_lora_linear_noalloc": (
         _int,
         [_p, _p, _int, _p, _int, _p, _int, _p, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _p],

@@ -1,0 +1,833 @@
+// The norms before and after a transformer block with its gate and residual
+// scale, forward and backward, for sm_100a. For each row of `cols` elements:
+//
+//   q = 1 / sqrt(mean(x^2) + eps)          p = x q post_weight  (p = x without post_weight)
+//   h = residual_scale residual + gate p   (gate = 1 without one)
+//   t = 1 / sqrt(mean(h^2) + eps)          n = h t weight
+//
+// x is the block's output, h the new residual stream, n the next block's input.
+// All of it is fp32; h and n are each rounded once (n from the unrounded h).
+// Backward, from dn and dh (either may be missing = zero), with xh = x q, hh = h t:
+//
+//   a  = dn weight                   m1 = mean(a hh)
+//   D  = dh + t (a - hh m1)          d residual = residual_scale D
+//   c  = gate D post_weight          m2 = mean(c xh)
+//   dx = q (c - xh m2)               (dx = gate D without post_weight)
+//   d weight = sum_rows dn hh, d post_weight = sum_rows gate D xh, d gate = sum D p
+//
+// HBM-bound: forward reads x and residual and writes n and h, backward reads x,
+// residual, dn and dh and writes dx and d residual; q and t are kept from the
+// forward pass (8 bytes a row), h is recomputed rather than read back rounded.
+// One row per group of kTpr threads, kPer elements of it in each thread's
+// registers through all passes, so nothing is read twice. Rows beyond the
+// register form (forward 16384 16-bit or 8192 fp32 elements, backward 8192)
+// take looping kernels that read their row again.
+//
+// The parameters' gradients are sums over rows. Each backward CTA walks a
+// fixed range of rows ("slot") and keeps its sums in registers; slots are
+// written as fp32 partials and a second launch adds them in a fixed order, so
+// results do not vary from run to run (no atomics).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "cf_common.cuh"
+
+namespace cfb {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// N consecutive elements moved as one access of up to 16 bytes at a time.
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+  T v[N];
+};
+
+// How a row is spread over threads: chunk i of thread t starts at column
+// (i * kTpr + t) * kVec, so a warp's accesses are contiguous.
+// Backward holds four values and up to three sums for each element: 8 of them
+// are about 80 registers, 16 spill at 512 threads and more.
+constexpr int kBackwardPer = 8;
+template <typename T>
+constexpr int kForwardPer = sizeof(T) == 4 ? 8 : 16;
+
+template <typename T, bool kWide, int kElems>
+struct Spread {
+  static constexpr int kPer = kElems;                              // elements per thread
+  static constexpr int kVec = kWide ? 16 / static_cast<int>(sizeof(T)) : 1;  // per access
+  static constexpr int kChunks = kPer / kVec;
+};
+
+template <typename T, int kVec>
+__device__ __forceinline__ void load_vec(const T *p, float *f) {
+  const Pack<T, kVec> v = *reinterpret_cast<const Pack<T, kVec> *>(p);
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) f[e] = to_float<T>(v.v[e]);
+}
+
+template <typename T, int kVec>
+__device__ __forceinline__ void store_vec(T *p, const float *f) {
+  Pack<T, kVec> v;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) v.v[e] = from_float<T>(f[e]);
+  *reinterpret_cast<Pack<T, kVec> *>(p) = v;
+}
+
+// Sum over the kTpr threads of a row. Groups of one warp need no barrier;
+// wider groups are the whole CTA and alternate between two buffers, so one
+// barrier per sum suffices (the next write of a buffer comes after the barrier
+// of the sum in between, which every reader of this one has passed).
+template <int kTpr>
+__device__ __forceinline__ float row_sum(float v, float (*buf)[32], int &parity) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (kTpr > kWarp) {
+    constexpr int kWarps = kTpr / kWarp;
+    const int lane = threadIdx.x & (kWarp - 1);
+    if (lane == 0) buf[parity][threadIdx.x / kWarp] = v;
+    __syncthreads();
+    v = lane < kWarps ? buf[parity][lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    parity ^= 1;
+  }
+  return v;
+}
+
+struct NormArgs {
+  const void *x, *residual, *weight, *post, *gate;
+  void *n, *h;
+  float *stats;  // [rows][2]: q and t, or null
+  int64_t rows, cols;
+  int64_t gate_rows;  // rows that share a row of the gate
+  float scale, eps;
+  // backward
+  const void *dn, *dh;
+  void *dx, *dres, *dgate;
+  float *part;  // partial sums: [3][slots][cols] (weight, post, gate)
+  float *means; // [rows][2]: m1 and m2 (long rows)
+  int64_t slots, group_chunks, rows_per_slot;
+  bool whole_groups;  // a slot holds whole gate groups and writes their gradients itself
+};
+
+constexpr int kThreadsSmall = 128;  // CTA of the warp-per-row form: four rows
+
+template <int kTpr>
+constexpr int cta_threads() { return kTpr == kWarp ? kThreadsSmall : kTpr; }
+
+// ---------------------------------------------------------------- forward
+
+template <typename T, typename TW, int kTpr, bool kWide>
+__global__ void __launch_bounds__(cta_threads<kTpr>())
+    gated_norm_kernel(const NormArgs a) {
+  using S = Spread<T, kWide, kForwardPer<T>>;
+  __shared__ float buf[2][32];
+  int parity = 0;
+  constexpr int kRows = cta_threads<kTpr>() / kTpr;
+  const int t = threadIdx.x % kTpr;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTpr;
+  if (row >= a.rows) return;  // whole warps, and only where a row is one warp
+  const int cols = static_cast<int>(a.cols);
+  const T *x = static_cast<const T *>(a.x) + row * a.cols;
+  const T *r = static_cast<const T *>(a.residual) + row * a.cols;
+  const TW *weight = static_cast<const TW *>(a.weight);
+  const TW *post = static_cast<const TW *>(a.post);
+  const TW *gate = a.gate ? static_cast<const TW *>(a.gate) + row / a.gate_rows * a.cols : nullptr;
+  float xv[S::kPer], rv[S::kPer];
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      load_vec<T, S::kVec>(x + c, xv + i * S::kVec);
+      load_vec<T, S::kVec>(r + c, rv + i * S::kVec);
+    } else {
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) xv[i * S::kVec + e] = rv[i * S::kVec + e] = 0.0f;
+    }
+  }
+  const float inv_cols = 1.0f / static_cast<float>(cols);
+  float q = 1.0f;
+  if (post != nullptr) {
+#pragma unroll
+    for (int e = 0; e < S::kPer; ++e) sum = fmaf(xv[e], xv[e], sum);
+    q = rsqrtf(row_sum<kTpr>(sum, buf, parity) * inv_cols + a.eps);
+  }
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      float *h = rv + i * S::kVec;
+      float p[S::kVec], w[S::kVec];
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) p[e] = xv[i * S::kVec + e] * q;
+      if (post != nullptr) {
+        load_vec<TW, S::kVec>(post + c, w);
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) p[e] *= w[e];
+      }
+      if (gate != nullptr) {
+        load_vec<TW, S::kVec>(gate + c, w);
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) p[e] *= w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) {
+        h[e] = fmaf(a.scale, h[e], p[e]);
+        sum = fmaf(h[e], h[e], sum);
+      }
+      store_vec<T, S::kVec>(static_cast<T *>(a.h) + row * a.cols + c, h);
+    }
+  }
+  const float rt = rsqrtf(row_sum<kTpr>(sum, buf, parity) * inv_cols + a.eps);
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      float w[S::kVec], n[S::kVec];
+      load_vec<TW, S::kVec>(weight + c, w);
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) n[e] = rv[i * S::kVec + e] * rt * w[e];
+      store_vec<T, S::kVec>(static_cast<T *>(a.n) + row * a.cols + c, n);
+    }
+  }
+  if (a.stats != nullptr && t == 0) {
+    a.stats[2 * row] = q;
+    a.stats[2 * row + 1] = rt;
+  }
+}
+
+// Element c of a row's residual sum, and of p, in fp32 (long rows: recomputed
+// in each pass).
+template <typename T, typename TW>
+__device__ __forceinline__ float sum_at(const NormArgs &a, const T *x, const T *r, const TW *gate,
+                                        int64_t c, float q, float &xh, float &p) {
+  xh = to_float<T>(x[c]) * q;
+  p = a.post ? xh * to_float<TW>(static_cast<const TW *>(a.post)[c]) : xh;
+  const float g = gate ? to_float<TW>(gate[c]) * p : p;
+  return fmaf(a.scale, to_float<T>(r[c]), g);
+}
+
+constexpr int kLongThreads = 1024;
+
+template <typename T, typename TW>
+__global__ void __launch_bounds__(kLongThreads) gated_norm_long_kernel(const NormArgs a) {
+  __shared__ float buf[2][32];
+  int parity = 0;
+  const int64_t row = blockIdx.x;
+  const T *x = static_cast<const T *>(a.x) + row * a.cols;
+  const T *r = static_cast<const T *>(a.residual) + row * a.cols;
+  const TW *weight = static_cast<const TW *>(a.weight);
+  const TW *gate = a.gate ? static_cast<const TW *>(a.gate) + row / a.gate_rows * a.cols : nullptr;
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  float q = 1.0f, sum = 0.0f, xh, p;
+  if (a.post != nullptr) {
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+      const float v = to_float<T>(x[c]);
+      sum = fmaf(v, v, sum);
+    }
+    q = rsqrtf(row_sum<kLongThreads>(sum, buf, parity) * inv_cols + a.eps);
+  }
+  sum = 0.0f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+    const float h = sum_at<T, TW>(a, x, r, gate, c, q, xh, p);
+    static_cast<T *>(a.h)[row * a.cols + c] = from_float<T>(h);
+    sum = fmaf(h, h, sum);
+  }
+  const float rt = rsqrtf(row_sum<kLongThreads>(sum, buf, parity) * inv_cols + a.eps);
+  for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+    const float h = sum_at<T, TW>(a, x, r, gate, c, q, xh, p);
+    static_cast<T *>(a.n)[row * a.cols + c] = from_float<T>(h * rt * to_float<TW>(weight[c]));
+  }
+  if (a.stats != nullptr && threadIdx.x == 0) {
+    a.stats[2 * row] = q;
+    a.stats[2 * row + 1] = rt;
+  }
+}
+
+// ---------------------------------------------------------------- backward
+
+// Rows [begin, end) of a slot. Either slots hold whole gate groups, or a group
+// is cut into group_chunks slots that stay inside it.
+__device__ __forceinline__ void slot_rows(const NormArgs &a, int64_t slot, int64_t group_rows,
+                                          int64_t &begin, int64_t &end) {
+  if (a.whole_groups) {
+    begin = slot * a.rows_per_slot;
+    end = min(a.rows, begin + a.rows_per_slot);
+  } else {
+    const int64_t group = slot / a.group_chunks;
+    const int64_t first = group * group_rows;
+    begin = min(first + (slot - group * a.group_chunks) * a.rows_per_slot, first + group_rows);
+    end = min(begin + a.rows_per_slot, first + group_rows);
+  }
+}
+
+// kShared: a row of the gate serves gate_rows > 1 rows, so its gradient is a
+// sum; otherwise there is none, or one for each row.
+template <typename T, typename TW, int kTpr, bool kWide, bool kShared>
+__global__ void __launch_bounds__(cta_threads<kTpr>())
+    gated_norm_backward_kernel(const NormArgs a) {
+  using S = Spread<T, kWide, kBackwardPer>;
+  __shared__ float buf[2][32];
+  int parity = 0;
+  constexpr int kSlots = cta_threads<kTpr>() / kTpr;
+  const int t = threadIdx.x % kTpr;
+  const int64_t slot = static_cast<int64_t>(blockIdx.x) * kSlots + threadIdx.x / kTpr;
+  if (slot >= a.slots) return;  // whole warps, and only where a row is one warp
+  const int cols = static_cast<int>(a.cols);
+  const float inv_cols = 1.0f / static_cast<float>(cols);
+  const TW *weight = static_cast<const TW *>(a.weight);
+  const TW *post = static_cast<const TW *>(a.post);
+  const int64_t group_rows = kShared ? a.gate_rows : a.rows;
+  int64_t begin, end;
+  slot_rows(a, slot, group_rows, begin, end);
+
+  float sum_w[S::kPer], sum_p[S::kPer], sum_g[S::kPer];
+#pragma unroll
+  for (int e = 0; e < S::kPer; ++e) sum_w[e] = sum_p[e] = sum_g[e] = 0.0f;
+
+  for (int64_t row = begin; row < end; ++row) {
+    const int64_t base = row * a.cols;
+    const TW *gate = a.gate == nullptr ? nullptr
+                                       : static_cast<const TW *>(a.gate) +
+                                             (kShared ? row / a.gate_rows : row) * a.cols;
+    const float q = a.stats[2 * row], rt = a.stats[2 * row + 1];
+    float xh[S::kPer], hh[S::kPer], av[S::kPer], dv[S::kPer];
+    float s1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      const int o = i * S::kVec;
+      if (c < cols) {
+        load_vec<T, S::kVec>(static_cast<const T *>(a.x) + base + c, xh + o);
+        load_vec<T, S::kVec>(static_cast<const T *>(a.residual) + base + c, hh + o);
+        if (a.dn) load_vec<T, S::kVec>(static_cast<const T *>(a.dn) + base + c, av + o);
+        if (a.dh) load_vec<T, S::kVec>(static_cast<const T *>(a.dh) + base + c, dv + o);
+      }
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) {
+        if (c >= cols) xh[o + e] = hh[o + e] = 0.0f;
+        if (c >= cols || !a.dn) av[o + e] = 0.0f;
+        if (c >= cols || !a.dh) dv[o + e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      if (c < cols) {
+        float w[S::kVec], p[S::kVec];
+        const int o = i * S::kVec;
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) p[e] = xh[o + e] = xh[o + e] * q;
+        if (post != nullptr) {
+          load_vec<TW, S::kVec>(post + c, w);
+#pragma unroll
+          for (int e = 0; e < S::kVec; ++e) p[e] *= w[e];
+        }
+        if (gate != nullptr) {
+          load_vec<TW, S::kVec>(gate + c, w);
+#pragma unroll
+          for (int e = 0; e < S::kVec; ++e) p[e] *= w[e];
+        }
+        load_vec<TW, S::kVec>(weight + c, w);
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) {
+          hh[o + e] = fmaf(a.scale, hh[o + e], p[e]) * rt;
+          sum_w[o + e] = fmaf(av[o + e], hh[o + e], sum_w[o + e]);
+          av[o + e] *= w[e];
+          s1 = fmaf(av[o + e], hh[o + e], s1);
+        }
+      }
+    }
+    const float m1 = row_sum<kTpr>(s1, buf, parity) * inv_cols;
+    float s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      if (c < cols) {
+        const int o = i * S::kVec;
+        float w[S::kVec], d[S::kVec], out[S::kVec];
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) {
+          d[e] = fmaf(rt, fmaf(-hh[o + e], m1, av[o + e]), dv[o + e]);
+          out[e] = a.scale * d[e];
+        }
+        store_vec<T, S::kVec>(static_cast<T *>(a.dres) + base + c, out);
+        float pw[S::kVec];
+        if (post != nullptr) load_vec<TW, S::kVec>(post + c, pw);
+        if (gate != nullptr) {
+          load_vec<TW, S::kVec>(gate + c, w);
+#pragma unroll
+          for (int e = 0; e < S::kVec; ++e) {
+            out[e] = d[e] * xh[o + e];
+            if (post != nullptr) out[e] *= pw[e];
+            if constexpr (kShared) sum_g[o + e] += out[e];
+            d[e] *= w[e];
+          }
+          if constexpr (!kShared) {
+            store_vec<TW, S::kVec>(static_cast<TW *>(a.dgate) + base + c, out);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) {
+          if (post != nullptr) {
+            sum_p[o + e] = fmaf(d[e], xh[o + e], sum_p[o + e]);
+            d[e] *= pw[e];
+            s2 = fmaf(d[e], xh[o + e], s2);
+          }
+          dv[o + e] = d[e];
+        }
+      }
+    }
+    float m2 = 0.0f;
+    if (post != nullptr) m2 = row_sum<kTpr>(s2, buf, parity) * inv_cols;
+    const bool group_done = kShared && a.whole_groups && (row + 1) % a.gate_rows == 0;
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      if (c < cols) {
+        const int o = i * S::kVec;
+        float out[S::kVec];
+#pragma unroll
+        for (int e = 0; e < S::kVec; ++e) {
+          out[e] = post != nullptr ? q * fmaf(-xh[o + e], m2, dv[o + e]) : dv[o + e];
+        }
+        store_vec<T, S::kVec>(static_cast<T *>(a.dx) + base + c, out);
+        if constexpr (kShared) {
+          if (group_done) {
+            store_vec<TW, S::kVec>(
+                static_cast<TW *>(a.dgate) + row / a.gate_rows * a.cols + c, sum_g + o);
+#pragma unroll
+            for (int e = 0; e < S::kVec; ++e) sum_g[o + e] = 0.0f;
+          }
+        }
+      }
+    }
+  }
+  // Partial sums; a slot without rows leaves zeros.
+  const int64_t plane = a.slots * a.cols;
+  float *part = a.part + slot * a.cols;
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+#pragma unroll
+    for (int e = 0; e < S::kVec; ++e) {
+      if (c + e < cols) {
+        part[c + e] = sum_w[i * S::kVec + e];
+        if (post != nullptr) part[plane + c + e] = sum_p[i * S::kVec + e];
+        if (kShared && !a.whole_groups) part[2 * plane + c + e] = sum_g[i * S::kVec + e];
+      }
+    }
+  }
+}
+
+// Long rows: m1 and m2 of each row with dx and d residual, then the columns'
+// sums in a kernel of their own.
+template <typename T, typename TW>
+__global__ void __launch_bounds__(kLongThreads) gated_norm_backward_long_kernel(const NormArgs a) {
+  __shared__ float buf[2][32];
+  int parity = 0;
+  const int64_t row = blockIdx.x;
+  const int64_t base = row * a.cols;
+  const T *x = static_cast<const T *>(a.x) + base;
+  const T *r = static_cast<const T *>(a.residual) + base;
+  const T *dn = a.dn ? static_cast<const T *>(a.dn) + base : nullptr;
+  const T *dh = a.dh ? static_cast<const T *>(a.dh) + base : nullptr;
+  const TW *weight = static_cast<const TW *>(a.weight);
+  const TW *post = static_cast<const TW *>(a.post);
+  const TW *gate = a.gate ? static_cast<const TW *>(a.gate) + row / a.gate_rows * a.cols : nullptr;
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const float q = a.stats[2 * row], rt = a.stats[2 * row + 1];
+  float s = 0.0f, m1 = 0.0f, m2 = 0.0f, xh, p;
+  if (dn) {
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+      const float hh = sum_at<T, TW>(a, x, r, gate, c, q, xh, p) * rt;
+      s = fmaf(to_float<T>(dn[c]) * to_float<TW>(weight[c]), hh, s);
+    }
+    m1 = row_sum<kLongThreads>(s, buf, parity) * inv_cols;
+  }
+  s = 0.0f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+      const float hh = sum_at<T, TW>(a, x, r, gate, c, q, xh, p) * rt;
+      const float av = dn ? to_float<T>(dn[c]) * to_float<TW>(weight[c]) : 0.0f;
+      float d = fmaf(rt, fmaf(-hh, m1, av), dh ? to_float<T>(dh[c]) : 0.0f);
+      if (pass == 0) {
+        static_cast<T *>(a.dres)[base + c] = from_float<T>(a.scale * d);
+        if (gate && a.gate_rows == 1) static_cast<TW *>(a.dgate)[base + c] = from_float<TW>(d * p);
+      }
+      if (gate) d *= to_float<TW>(gate[c]);
+      if (post) d *= to_float<TW>(post[c]);
+      if (pass == 0) {
+        s = fmaf(d, xh, s);
+      } else {
+        static_cast<T *>(a.dx)[base + c] =
+            from_float<T>(post ? q * fmaf(-xh, m2, d) : d);
+      }
+    }
+    if (pass == 0 && post) m2 = row_sum<kLongThreads>(s, buf, parity) * inv_cols;
+  }
+  if (threadIdx.x == 0) {
+    a.means[2 * row] = m1;
+    a.means[2 * row + 1] = m2;
+  }
+}
+
+constexpr int kColumnThreads = 256;
+
+template <typename T, typename TW>
+__global__ void __launch_bounds__(kColumnThreads)
+    gated_norm_backward_columns_kernel(const NormArgs a) {
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kColumnThreads + threadIdx.x;
+  if (c >= a.cols) return;
+  const bool shared_gate = a.gate != nullptr && a.gate_rows > 1;
+  const int64_t slot = blockIdx.y;
+  int64_t begin, end;
+  slot_rows(a, slot, shared_gate ? a.gate_rows : a.rows, begin, end);
+  float sum_w = 0.0f, sum_p = 0.0f, sum_g = 0.0f;
+  const float w = to_float<TW>(static_cast<const TW *>(a.weight)[c]);
+  for (int64_t row = begin; row < end; ++row) {
+    const int64_t base = row * a.cols;
+    const TW *gate =
+        a.gate ? static_cast<const TW *>(a.gate) + row / a.gate_rows * a.cols : nullptr;
+    const float q = a.stats[2 * row], rt = a.stats[2 * row + 1];
+    float xh, p;
+    const float hh = sum_at<T, TW>(a, static_cast<const T *>(a.x) + base,
+                                   static_cast<const T *>(a.residual) + base, gate, c, q, xh, p) *
+                     rt;
+    const float dn = a.dn ? to_float<T>(static_cast<const T *>(a.dn)[base + c]) : 0.0f;
+    const float dh = a.dh ? to_float<T>(static_cast<const T *>(a.dh)[base + c]) : 0.0f;
+    const float d = fmaf(rt, fmaf(-hh, a.means[2 * row], dn * w), dh);
+    sum_w = fmaf(dn, hh, sum_w);
+    sum_g = fmaf(d, p, sum_g);
+    sum_p = fmaf(gate ? d * to_float<TW>(gate[c]) : d, xh, sum_p);
+    if (shared_gate && a.whole_groups && (row + 1) % a.gate_rows == 0) {
+      static_cast<TW *>(a.dgate)[row / a.gate_rows * a.cols + c] = from_float<TW>(sum_g);
+      sum_g = 0.0f;
+    }
+  }
+  const int64_t plane = a.slots * a.cols;
+  float *part = a.part + slot * a.cols + c;
+  part[0] = sum_w;
+  if (a.post) part[plane] = sum_p;
+  if (shared_gate && !a.whole_groups) part[2 * plane] = sum_g;
+}
+
+// Adds the slots' partial sums. blockIdx.y: 0 weight, 1 post_weight, 2 + g the
+// gate's group g. A thread adds every kFinishRows-th slot, in order.
+constexpr int kFinishCols = 32, kFinishRows = 16;
+
+template <typename TW>
+__global__ void __launch_bounds__(kFinishCols *kFinishRows)
+    gated_norm_finish_kernel(const float *part, int64_t slots, int64_t cols, int64_t group_chunks,
+                             TW *dweight, TW *dpost, TW *dgate) {
+  __shared__ float sums[kFinishRows][kFinishCols + 1];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kFinishCols + threadIdx.x;
+  const int64_t which = blockIdx.y;
+  TW *out = which == 0 ? dweight : which == 1 ? dpost : dgate + (which - 2) * cols;
+  if (which == 1 && dpost == nullptr) return;
+  const int64_t first = which < 2 ? 0 : (which - 2) * group_chunks;
+  const int64_t count = which < 2 ? slots : group_chunks;
+  const float *src = part + (min(which, int64_t{2}) * slots + first) * cols + c;
+  float s = 0.0f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int64_t k = threadIdx.y; k < count; k += kFinishRows) s += src[k * cols];
+  }
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+    float total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFinishRows; ++k) total += sums[k][threadIdx.x];
+    out[c] = from_float<TW>(total);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// Threads for a row of `cols` elements at `per` elements a thread; 0: long row.
+int threads_per_row(int64_t cols, int per) {
+  for (int tpr : {32, 128, 256, 512, 1024}) {
+    if (cols <= static_cast<int64_t>(tpr) * per) return tpr;
+  }
+  return 0;
+}
+
+
+// The backward pass's slots: about as many rows at a time as an SM holds (512
+// threads of them), since more only add partial sums.
+void plan_slots(NormArgs &a, bool shared_gate) {
+  const int tpr = threads_per_row(a.cols, kBackwardPer);
+  const int64_t per_sm = tpr == 0 ? 2 : std::max(1, 512 / tpr);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.rows, per_sm * sm_count()));
+  const int64_t group_rows = shared_gate ? a.gate_rows : a.rows;
+  const int64_t groups = a.rows / group_rows;
+  if (shared_gate && groups >= want) {
+    a.whole_groups = true;
+    a.group_chunks = 1;
+    const int64_t per_slot = (groups + want - 1) / want;
+    a.rows_per_slot = per_slot * group_rows;
+    a.slots = (groups + per_slot - 1) / per_slot;
+  } else {
+    a.whole_groups = false;
+    a.group_chunks = std::min(group_rows, std::max<int64_t>(1, want / groups));
+    a.rows_per_slot = (group_rows + a.group_chunks - 1) / a.group_chunks;
+    a.group_chunks = (group_rows + a.rows_per_slot - 1) / a.rows_per_slot;
+    a.slots = groups * a.group_chunks;
+  }
+}
+
+size_t part_bytes(const NormArgs &a, bool post, bool shared_gate) {
+  const size_t planes = shared_gate && !a.whole_groups ? 3 : post ? 2 : 1;
+  const size_t bytes = planes * static_cast<size_t>(a.slots) * static_cast<size_t>(a.cols) * 4;
+  return (bytes + 255) & ~static_cast<size_t>(255);
+}
+
+template <typename T, typename TW, int kTpr>
+int launch_forward(const NormArgs &a, bool wide, cudaStream_t s) {
+  constexpr int kRows = cta_threads<kTpr>() / kTpr;
+  const unsigned grid = static_cast<unsigned>((a.rows + kRows - 1) / kRows);
+  if (wide) {
+    gated_norm_kernel<T, TW, kTpr, true><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
+  } else {
+    gated_norm_kernel<T, TW, kTpr, false><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
+  }
+  return check_launch();
+}
+
+template <typename T, typename TW>
+int forward(const NormArgs &a, bool wide, cudaStream_t s) {
+  switch (threads_per_row(a.cols, kForwardPer<T>)) {
+    case 32: return launch_forward<T, TW, 32>(a, wide, s);
+    case 128: return launch_forward<T, TW, 128>(a, wide, s);
+    case 256: return launch_forward<T, TW, 256>(a, wide, s);
+    case 512: return launch_forward<T, TW, 512>(a, wide, s);
+    case 1024: return launch_forward<T, TW, 1024>(a, wide, s);
+    default:
+      gated_norm_long_kernel<T, TW>
+          <<<static_cast<unsigned>(a.rows), kLongThreads, 0, s>>>(a);
+      return check_launch();
+  }
+}
+
+template <typename T, typename TW, int kTpr, bool kWide>
+int launch_backward(const NormArgs &a, cudaStream_t s) {
+  constexpr int kSlots = cta_threads<kTpr>() / kTpr;
+  const unsigned grid = static_cast<unsigned>((a.slots + kSlots - 1) / kSlots);
+  constexpr int kThreads = cta_threads<kTpr>();
+  if (a.gate != nullptr && a.gate_rows > 1) {
+    gated_norm_backward_kernel<T, TW, kTpr, kWide, true><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    gated_norm_backward_kernel<T, TW, kTpr, kWide, false><<<grid, kThreads, 0, s>>>(a);
+  }
+  return check_launch();
+}
+
+template <typename T, typename TW>
+int backward(const NormArgs &a, bool wide, void *dweight, void *dpost, cudaStream_t s) {
+  int st = CF_OK;
+  switch (threads_per_row(a.cols, kBackwardPer)) {
+#define CFB_CASE(tpr)                                                  \
+  case tpr:                                                            \
+    st = wide ? launch_backward<T, TW, tpr, true>(a, s)                \
+              : launch_backward<T, TW, tpr, false>(a, s);              \
+    break
+    CFB_CASE(32);
+    CFB_CASE(128);
+    CFB_CASE(256);
+    CFB_CASE(512);
+    CFB_CASE(1024);
+#undef CFB_CASE
+    default: {
+      gated_norm_backward_long_kernel<T, TW>
+          <<<static_cast<unsigned>(a.rows), kLongThreads, 0, s>>>(a);
+      if ((st = check_launch()) != CF_OK) return st;
+      const dim3 grid(static_cast<unsigned>((a.cols + kColumnThreads - 1) / kColumnThreads),
+                      static_cast<unsigned>(a.slots));
+      gated_norm_backward_columns_kernel<T, TW><<<grid, kColumnThreads, 0, s>>>(a);
+      st = check_launch();
+    }
+  }
+  if (st != CF_OK) return st;
+  const bool gate_parts = a.gate != nullptr && a.gate_rows > 1 && !a.whole_groups;
+  const dim3 grid(static_cast<unsigned>((a.cols + kFinishCols - 1) / kFinishCols),
+                  static_cast<unsigned>(2 + (gate_parts ? a.slots / a.group_chunks : 0)));
+  gated_norm_finish_kernel<TW><<<grid, dim3(kFinishCols, kFinishRows), 0, s>>>(
+      a.part, a.slots, a.cols, a.group_chunks, static_cast<TW *>(dweight),
+      static_cast<TW *>(dpost), static_cast<TW *>(a.dgate));
+  return check_launch();
+}
+
+template <bool kForward>
+int dispatch_norm(const NormArgs &a, int dtype, int weight_dtype, bool wide, void *dweight, void *dpost,
+             cudaStream_t s) {
+  const bool wf = weight_dtype == CF_DTYPE_F32;
+#define CFB_RUN(T, TW)                                       \
+  do {                                                       \
+    if constexpr (kForward) {                                \
+      return forward<T, TW>(a, wide, s);                     \
+    } else {                                                 \
+      return backward<T, TW>(a, wide, dweight, dpost, s);    \
+    }                                                        \
+  } while (0)
+  switch (dtype) {
+    case CF_DTYPE_F32: CFB_RUN(float, float);
+    case CF_DTYPE_BF16:
+      if (wf) CFB_RUN(__nv_bfloat16, float);
+      CFB_RUN(__nv_bfloat16, __nv_bfloat16);
+    default:
+      if (wf) CFB_RUN(__half, float);
+      CFB_RUN(__half, __half);
+  }
+#undef CFB_RUN
+}
+
+// Checks shared by both directions.
+int check_norm_args(int64_t rows, int64_t cols, int64_t gate_groups, bool gate, int dtype,
+                    int weight_dtype) {
+  if (rows < 0 || cols < 0 || gate_groups < 1) return CF_ERR_INVALID_ARGUMENT;
+  if (dtype != CF_DTYPE_F32 && dtype != CF_DTYPE_BF16 && dtype != CF_DTYPE_F16) {
+    return CF_ERR_UNSUPPORTED;
+  }
+  if (weight_dtype != dtype && weight_dtype != CF_DTYPE_F32) return CF_ERR_UNSUPPORTED;
+  if (rows == 0 || cols == 0) return CF_OK;
+  if (gate && rows % gate_groups != 0) return CF_ERR_INVALID_ARGUMENT;
+  // Grid dimensions: rows in x, gate groups and slots in y.
+  if (rows > 0x7fffffffll || cols > (int64_t{1} << 40) / rows) return CF_ERR_INVALID_ARGUMENT;
+  return CF_OK;
+}
+
+bool wide_rows(int64_t cols, int dtype, std::initializer_list<const void *> pointers) {
+  if (cols % (dtype == CF_DTYPE_F32 ? 4 : 8) != 0) return false;
+  for (const void *p : pointers) {
+    if (!aligned_to(p, 16)) return false;  // a null pointer is aligned
+  }
+  return true;
+}
+
+}  // namespace
+}  // namespace cfb
+
+extern "C" {
+
+int cf_gated_residual_rmsnorm(const void *x, const void *residual, const void *weight,
+                              const void *post_weight, const void *gate, int64_t gate_groups,
+                              int weight_dtype, void *normalised, void *residual_out, float *stats,
+                              int64_t rows, int64_t cols, float residual_scale, float eps,
+                              int dtype, cf_stream_t stream) {
+  if (int st = cfb::check_norm_args(rows, cols, gate_groups, gate != nullptr, dtype,
+                                    weight_dtype)) {
+    return st;
+  }
+  if (rows == 0 || cols == 0) return CF_OK;
+  if (!x || !residual || !weight || !normalised || !residual_out) return CF_ERR_INVALID_ARGUMENT;
+  cfb::NormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.post = post_weight;
+  a.gate = gate;
+  a.gate_rows = gate ? rows / gate_groups : rows;
+  a.n = normalised;
+  a.h = residual_out;
+  a.stats = stats;
+  a.rows = rows;
+  a.cols = cols;
+  a.scale = residual_scale;
+  a.eps = eps;
+  const bool wide = cfb::wide_rows(
+      cols, dtype, {x, residual, weight, post_weight, gate, normalised, residual_out});
+  return cfb::dispatch_norm<true>(a, dtype, weight_dtype, wide, nullptr, nullptr,
+                             reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t cf_gated_residual_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t cols,
+                                                          int has_post_weight,
+                                                          int64_t gate_groups) {
+  if (rows <= 0 || cols <= 0 || (gate_groups > 0 && rows % gate_groups != 0)) return 0;
+  cfb::NormArgs a{};
+  a.rows = rows;
+  a.cols = cols;
+  const bool shared = gate_groups > 0 && gate_groups < rows;
+  a.gate_rows = gate_groups > 0 ? rows / gate_groups : rows;
+  cfb::plan_slots(a, shared);
+  size_t bytes = cfb::part_bytes(a, has_post_weight != 0, shared);
+  if (cfb::threads_per_row(cols, cfb::kBackwardPer) == 0) {
+    bytes += static_cast<size_t>(rows) * 2 * sizeof(float);
+  }
+  return bytes;
+}
+
+int cf_gated_residual_rmsnorm_backward(
+    const void *d_normalised, const void *d_residual_out, const void *x, const void *residual,
+    const void *weight, const void *post_weight, const void *gate, int64_t gate_groups,
+    int weight_dtype, const float *stats, void *dx, void *d_residual, void *d_weight,
+    void *d_post_weight, void *d_gate, int64_t rows, int64_t cols, float residual_scale, int dtype,
+    void *workspace, size_t workspace_bytes, cf_stream_t stream) {
+  if (int st = cfb::check_norm_args(rows, cols, gate_groups, gate != nullptr, dtype,
+                                    weight_dtype)) {
+    return st;
+  }
+  if (rows == 0 || cols == 0) return CF_OK;
+  if (!x || !residual || !weight || !stats || !dx || !d_residual || !d_weight ||
+      (d_post_weight == nullptr) != (post_weight == nullptr) ||
+      (d_gate == nullptr) != (gate == nullptr)) {
+    return CF_ERR_INVALID_ARGUMENT;
+  }
+  cfb::NormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.post = post_weight;
+  a.gate = gate;
+  a.gate_rows = gate ? rows / gate_groups : rows;
+  a.stats = const_cast<float *>(stats);
+  a.rows = rows;
+  a.cols = cols;
+  a.scale = residual_scale;
+  a.dn = d_normalised;
+  a.dh = d_residual_out;
+  a.dx = dx;
+  a.dres = d_residual;
+  a.dgate = d_gate;
+  const bool shared = gate != nullptr && a.gate_rows > 1;
+  cfb::plan_slots(a, shared);
+  const size_t need = cf_gated_residual_rmsnorm_backward_workspace_bytes(
+      rows, cols, post_weight != nullptr, gate ? gate_groups : 0);
+  if (workspace == nullptr || workspace_bytes < need) return CF_ERR_WORKSPACE;
+  if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
+  a.part = static_cast<float *>(workspace);
+  a.means = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                      cfb::part_bytes(a, post_weight != nullptr, shared));
+  const bool wide = cfb::wide_rows(cols, dtype,
+                                   {x, residual, weight, post_weight, gate, dx, d_residual,
+                                    d_normalised, d_residual_out, d_gate});
+  return cfb::dispatch_norm<false>(a, dtype, weight_dtype, wide, d_weight, d_post_weight,
+                              reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -7,7 +7,8 @@
 // dequantize_int8, lora_linear, rmsnorm, fused_residual_rmsnorm) the CUDA key
 // runs this build's sm_100a kernels through the C ABI; the other five keep the
 // reference's semantics as ATen compositions (see below). The Autograd key raises
-// (autogradNotImplementedFallback), as the reference does (bindings.cpp:369-377).
+// (autogradNotImplementedFallback), as the reference does (bindings.cpp:369-377),
+// except for the additive ops that have a backward pass.
 //
 // CPU tensors: the reference's extension registers ATen CPU kernels for its
 // schemas (bindings.cpp:379-390), and its Python wrapper sends CPU tensors to
@@ -25,9 +26,12 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
+#include <optional>
+#include <utility>
 #include <vector>
 
 #include "cudaforge_b200.h"
@@ -338,6 +342,191 @@ std::vector<at::Tensor> fused_residual_rmsnorm_cuda(const at::Tensor &x, const a
   return {out, summed};
 }
 
+// The norms around a block. x and residual may have any leading dimensions; the
+// gate's leading dimensions have been reduced to `gate_groups` rows by the
+// Python wrapper. Parameters of mixed dtypes are read in float32.
+struct BlockNormParams {
+  at::Tensor weight, post, gate;
+  int dtype;
+};
+
+const void *data_or_null(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+BlockNormParams block_norm_params(const at::Tensor &x, const at::Tensor &residual,
+                                  const at::Tensor &weight,
+                                  const std::optional<at::Tensor> &post_weight,
+                                  const std::optional<at::Tensor> &gate, int64_t gate_groups) {
+  check_cuda(x, "x");
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  check_contiguous(x, "x");
+  check_contiguous(residual, "residual");
+  TORCH_CHECK(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type() &&
+                  residual.device() == x.device(),
+              "residual must have x's shape, dtype and device");
+  dtype_code(x, "x");
+  const int64_t cols = x.size(-1);
+  BlockNormParams p{weight, post_weight.value_or(at::Tensor()), gate.value_or(at::Tensor()), 0};
+  bool same = true;
+  for (const auto &[t, name] : {std::pair<at::Tensor *, const char *>{&p.weight, "weight"},
+                                {&p.post, "post_weight"}, {&p.gate, "gate"}}) {
+    if (!t->defined()) continue;
+    dtype_code(*t, name);
+    check_contiguous(*t, name);
+    TORCH_CHECK(t->device() == x.device(), name, " must be on x's device");
+    TORCH_CHECK(t->numel() == (t == &p.gate ? gate_groups : 1) * cols, name, " has ", t->numel(),
+                " elements, not ", (t == &p.gate ? gate_groups : 1) * cols);
+    same = same && t->scalar_type() == x.scalar_type();
+  }
+  if (!same) {
+    for (at::Tensor *t : {&p.weight, &p.post, &p.gate}) {
+      if (t->defined()) *t = t->to(at::kFloat);
+    }
+  }
+  p.dtype = dtype_code(p.weight, "weight");
+  return p;
+}
+
+// normalised and residual_out, and with `with_stats` the rows' statistics.
+std::vector<at::Tensor> block_norm_forward(const at::Tensor &x, const at::Tensor &residual,
+                                           const at::Tensor &weight,
+                                           const std::optional<at::Tensor> &post_weight,
+                                           const std::optional<at::Tensor> &gate,
+                                           int64_t gate_groups, double residual_scale, double eps,
+                                           bool with_stats) {
+  check_cuda(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const BlockNormParams p = block_norm_params(x, residual, weight, post_weight, gate, gate_groups);
+  const int64_t cols = x.size(-1), rows = cols > 0 ? x.numel() / cols : 0;
+  std::vector<at::Tensor> out{at::empty_like(x), at::empty_like(x)};
+  float *stats = nullptr;
+  if (with_stats) {
+    out.push_back(at::empty({rows, 2}, x.options().dtype(at::kFloat)));
+    stats = out[2].data_ptr<float>();
+  }
+  check_status(cf_gated_residual_rmsnorm(
+                   x.const_data_ptr(), residual.const_data_ptr(), data_or_null(p.weight),
+                   data_or_null(p.post), data_or_null(p.gate), gate_groups, p.dtype,
+                   out[0].data_ptr(), out[1].data_ptr(), stats, rows, cols,
+                   static_cast<float>(residual_scale), static_cast<float>(eps),
+                   dtype_code(x, "x"), current_stream()),
+               "gated_residual_rmsnorm");
+  return out;
+}
+
+std::vector<at::Tensor> gated_residual_rmsnorm_cuda(
+    const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight,
+    const std::optional<at::Tensor> &post_weight, const std::optional<at::Tensor> &gate,
+    int64_t gate_groups, double residual_scale, double eps) {
+  return block_norm_forward(x, residual, weight, post_weight, gate, gate_groups, residual_scale,
+                            eps, false);
+}
+
+// Gradients of x, residual, weight, post_weight and gate in their own dtypes; an
+// absent parameter's is undefined.
+std::vector<at::Tensor> block_norm_backward(
+    at::Tensor dn, at::Tensor dh, const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight,
+    const std::optional<at::Tensor> &post_weight, const std::optional<at::Tensor> &gate,
+    int64_t gate_groups, double residual_scale, const at::Tensor &stats) {
+  check_cuda(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const BlockNormParams p = block_norm_params(x, residual, weight, post_weight, gate, gate_groups);
+  const int64_t cols = x.size(-1), rows = cols > 0 ? x.numel() / cols : 0;
+  for (at::Tensor *t : {&dn, &dh}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(t->sizes() == x.sizes() && t->scalar_type() == x.scalar_type() &&
+                    t->device() == x.device(),
+                "incoming gradients must have x's shape, dtype and device");
+    *t = t->contiguous();
+  }
+  const bool empty = x.numel() == 0;
+  auto like = [&](const at::Tensor &t) {
+    if (!t.defined()) return at::Tensor();
+    return empty ? at::zeros_like(t) : at::empty_like(t);
+  };
+  std::vector<at::Tensor> out{at::empty_like(x), at::empty_like(x), like(p.weight), like(p.post),
+                              like(p.gate)};
+  auto typed = [&] {  // parameters' gradients in the parameters' dtypes
+    const at::Tensor none;
+    const at::Tensor *const to[] = {&weight, post_weight ? &*post_weight : &none,
+                                    gate ? &*gate : &none};
+    for (int i = 0; i < 3; ++i) {
+      if (out[2 + i].defined()) out[2 + i] = out[2 + i].to(to[i]->scalar_type());
+    }
+    return out;
+  };
+  if (empty) return typed();
+  const int dtype = dtype_code(x, "x");
+  const size_t ws_bytes = cf_gated_residual_rmsnorm_backward_workspace_bytes(
+      rows, cols, p.post.defined(), p.gate.defined() ? gate_groups : 0);
+  at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+  check_status(
+      cf_gated_residual_rmsnorm_backward(
+          data_or_null(dn), data_or_null(dh), x.const_data_ptr(), residual.const_data_ptr(),
+          data_or_null(p.weight), data_or_null(p.post), data_or_null(p.gate), gate_groups, p.dtype,
+          stats.data_ptr<float>(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+          p.post.defined() ? out[3].data_ptr() : nullptr,
+          p.gate.defined() ? out[4].data_ptr() : nullptr, rows, cols,
+          static_cast<float>(residual_scale), dtype, ws.data_ptr(), ws_bytes, current_stream()),
+      "gated_residual_rmsnorm_backward");
+  return typed();
+}
+
+// A gradient of a gradient would need the formulas' derivatives, which the
+// kernels do not have: refused rather than taken as constant.
+void check_differentiated_once(const char *op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op,
+              ": gradients of gradients are not implemented (create_graph=True)");
+}
+
+struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &residual,
+      const at::Tensor &weight, const std::optional<at::Tensor> &post_weight,
+      const std::optional<at::Tensor> &gate, int64_t gate_groups, double residual_scale,
+      double eps) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    std::vector<at::Tensor> out = block_norm_forward(x, residual, weight, post_weight, gate,
+                                                     gate_groups, residual_scale, eps, true);
+    ctx->save_for_backward({x, residual, weight, post_weight.value_or(at::Tensor()),
+                            gate.value_or(at::Tensor()), out[2]});
+    ctx->saved_data["gate_groups"] = gate_groups;
+    ctx->saved_data["residual_scale"] = residual_scale;
+    ctx->set_materialize_grads(false);
+    return {out[0], out[1]};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    if (!grads[0].defined() && !grads[1].defined()) return torch::autograd::variable_list(8);
+    check_differentiated_once("gated_residual_rmsnorm");
+    const auto saved = ctx->get_saved_variables();
+    auto optional = [](const at::Tensor &t) {
+      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    };
+    std::vector<at::Tensor> out = block_norm_backward(
+        grads[0], grads[1], saved[0], saved[1], saved[2], optional(saved[3]), optional(saved[4]),
+        ctx->saved_data["gate_groups"].toInt(), ctx->saved_data["residual_scale"].toDouble(),
+        saved[5]);
+    out.resize(8);
+    return out;
+  }
+};
+
+std::vector<at::Tensor> gated_residual_rmsnorm_autograd(
+    const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight,
+    const std::optional<at::Tensor> &post_weight, const std::optional<at::Tensor> &gate,
+    int64_t gate_groups, double residual_scale, double eps) {
+  auto wants = [](const std::optional<at::Tensor> &t) { return t && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (x.requires_grad() || residual.requires_grad() ||
+                                     weight.requires_grad() || wants(post_weight) || wants(gate))) {
+    return BlockNormFunction::apply(x, residual, weight, post_weight, gate, gate_groups,
+                                    residual_scale, eps);
+  }
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return gated_residual_rmsnorm_cuda(x, residual, weight, post_weight, gate, gate_groups,
+                                     residual_scale, eps);
+}
+
 // ---- host tensors: the reference semantics (python/cudaforge/ops.py:164-240)
 
 std::vector<at::Tensor> quantize_int8_host(const at::Tensor &input) {
@@ -438,6 +627,9 @@ TORCH_LIBRARY(cudaforge, m) {
       "float scale) -> Tensor");
   m.def("quantize_dequantize(Tensor input) -> Tensor");
   m.def("quantize_int8_many(Tensor[] inputs) -> Tensor[]");
+  m.def(
+      "gated_residual_rmsnorm(Tensor x, Tensor residual, Tensor weight, Tensor? post_weight, "
+      "Tensor? gate, int gate_groups, float residual_scale, float eps) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
@@ -447,6 +639,7 @@ TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
                            "swiglu"}) {
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
   }
+  m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_autograd);
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
@@ -458,6 +651,7 @@ TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
   m.impl("quantize_int8_many", &quantize_int8_many_cuda);
   m.impl("rmsnorm", &rmsnorm_cuda);
   m.impl("fused_residual_rmsnorm", &fused_residual_rmsnorm_cuda);
+  m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_cuda);
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CompositeExplicitAutograd, m) {

@@ -23,11 +23,14 @@ three differences that are deliberate:
 the reference's names, arguments and messages and take all three dtypes.
 
 Additive ops: ``lora_linear_int8`` (W as block-INT8 codes + scales),
-``quantize_dequantize`` (fake quantisation) and ``quantize_int8_many``.
+``quantize_dequantize`` (fake quantisation), ``quantize_int8_many`` and, around a
+transformer's feed-forward block, ``gated_residual_rmsnorm``, which is
+differentiable.
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -97,12 +100,16 @@ def kernel_supports(dtype: torch.dtype) -> bool:
     return dtype in KERNEL_DTYPES
 
 
-def _require(op: str, *tensors: torch.Tensor) -> None:
+def _require_cuda(op: str, *tensors: torch.Tensor | None) -> None:
     if not _EXTENSION_LOADED:
         raise RuntimeError(f"{op}: {_LOAD_MESSAGE}")
     for t in tensors:
-        if not t.is_cuda:
+        if t is not None and not t.is_cuda:
             raise RuntimeError(f"{op}: CUDA tensors required (this build has no CPU path)")
+
+
+def _require(op: str, *tensors: torch.Tensor) -> None:
+    _require_cuda(op, *tensors)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{op}: inference-only kernels; no backward is implemented")
 
@@ -198,6 +205,78 @@ def fused_residual_rmsnorm(
         x.contiguous().view(-1, hidden), residual.contiguous().view(-1, hidden),
         weight.contiguous(), float(eps))
     return normalised.view(x.shape), summed.view(x.shape)
+
+
+def _gate_groups(x: torch.Tensor, gate: torch.Tensor) -> int:
+    """Rows of the gate, each serving an equal run of x's rows."""
+    shape, hidden = tuple(x.shape), x.shape[-1]
+    if tuple(gate.shape) == (hidden,):
+        return 1
+    if gate.ndim == x.ndim and gate.shape[-1] == hidden:
+        lead = tuple(gate.shape[:-1])
+        kept = len(lead)
+        while kept and lead[kept - 1] == 1:
+            kept -= 1
+        if lead[:kept] == shape[:kept]:
+            return max(1, math.prod(lead))
+    raise ValueError(
+        f"gate must be [{hidden}], or x's shape with trailing dimensions before the last set "
+        f"to 1; got {tuple(gate.shape)} for x {shape}"
+    )
+
+
+def gated_residual_rmsnorm(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    residual_scale: float = 1.0,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The norms after and before a block, its gate and its residual add, in one pass.
+
+    With ``x`` the block's output and ``residual`` the stream it was computed from::
+
+        p            = rmsnorm(x, post_weight)            (x itself without post_weight)
+        residual_out = residual_scale * residual + gate * p
+        normalised   = rmsnorm(residual_out, weight)
+
+    in fp32, ``residual_out`` and ``normalised`` each rounded once to x's dtype
+    (``normalised`` from the unrounded sum, unlike
+    :func:`fused_residual_rmsnorm`, which keeps the reference's rounding in
+    between). Returns ``(normalised, residual_out)``.
+
+    Args:
+        x, residual: ``[..., hidden]`` of one float dtype.
+        weight, post_weight: ``[hidden]`` of any float dtype.
+        gate: ``[hidden]``, x's shape, or x's shape with trailing dimensions
+            before the last set to 1 (``[batch, 1, hidden]``: a gate for each
+            sample of ``[batch, tokens, hidden]``).
+        residual_scale: a number.
+
+    Differentiable in every tensor, once. Gradients of ``weight``,
+    ``post_weight`` and ``gate`` are summed over rows in fp32 in a fixed order.
+    """
+    if x.ndim < 1 or x.shape != residual.shape:
+        raise ValueError(
+            f"x and residual must have the same shape, got {tuple(x.shape)} "
+            f"and {tuple(residual.shape)}"
+        )
+    if x.dtype != residual.dtype or x.dtype not in KERNEL_DTYPES:
+        raise ValueError("x and residual must share one dtype of float32, float16 and bfloat16, "
+                         f"got {x.dtype} and {residual.dtype}")
+    hidden = x.shape[-1]
+    for name, w in (("weight", weight), ("post_weight", post_weight)):
+        if w is not None and (w.ndim != 1 or w.shape[0] != hidden):
+            raise ValueError(f"{name} must be 1-D of length {hidden}, got {tuple(w.shape)}")
+    groups = 1 if gate is None else _gate_groups(x, gate)
+    _require_cuda("gated_residual_rmsnorm", x, residual, weight, post_weight, gate)
+    normalised, residual_out = torch.ops.cudaforge.gated_residual_rmsnorm(
+        x.contiguous(), residual.contiguous(), weight.contiguous(),
+        None if post_weight is None else post_weight.contiguous(),
+        None if gate is None else gate.contiguous(), groups, float(residual_scale), float(eps))
+    return normalised, residual_out
 
 
 def matmul_f32(a: torch.Tensor, b: torch.Tensor, precise: bool = True) -> torch.Tensor:

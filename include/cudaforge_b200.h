@@ -291,6 +291,44 @@ CF_API int cf_fused_residual_rmsnorm(const void *x, const void *residual, const 
                                      int64_t rows, int64_t cols, float eps, int dtype,
                                      cf_stream_t stream);
 
+/* The norms before and after a transformer block with its gate and residual
+ * scale, one pass over the rows (rows x cols, contiguous):
+ *   p = x / sqrt(mean(x^2) + eps) * post_weight     (p = x when post_weight is NULL)
+ *   h = residual_scale * residual + gate * p        (gate = 1 when NULL)
+ *   normalised = h / sqrt(mean(h^2) + eps) * weight
+ * in fp32; residual_out = h and normalised are each rounded once to dtype
+ * (normalised from the unrounded h). gate is [gate_groups, cols]: group g holds
+ * rows [g * rows / gate_groups, ...), so 1 is a gate for each channel and rows a
+ * gate for each element; rows % gate_groups == 0. weight, post_weight and gate
+ * are of weight_dtype, which is dtype or f32. stats, float [rows][2], receives
+ * what the backward pass needs, or is NULL. Any alignment works; 16-byte aligned
+ * pointers and rows of whole 16-byte units take the vector path. No counterpart
+ * in the reference, whose fused_residual_rmsnorm (cuda/include/cudaforge/
+ * fused_norm.cuh) has neither post-norm, gate, scale nor a backward pass. */
+CF_API int cf_gated_residual_rmsnorm(const void *x, const void *residual, const void *weight,
+                                     const void *post_weight, const void *gate,
+                                     int64_t gate_groups, int weight_dtype, void *normalised,
+                                     void *residual_out, float *stats, int64_t rows, int64_t cols,
+                                     float residual_scale, float eps, int dtype,
+                                     cf_stream_t stream);
+
+/* Gradients of cf_gated_residual_rmsnorm for d_normalised and d_residual_out
+ * (either may be NULL: zero), from the forward call's inputs and stats. dx and
+ * d_residual [rows, cols] are of dtype; d_weight, d_post_weight [cols] (NULL
+ * exactly when post_weight is) and d_gate [gate_groups, cols] (NULL exactly when
+ * gate is) of weight_dtype, summed over rows in fp32 in a fixed order.
+ * Workspace: cf_gated_residual_rmsnorm_backward_workspace_bytes (gate_groups 0
+ * for no gate) bytes of device memory, 16-byte aligned. rows == 0 writes nothing. */
+CF_API size_t cf_gated_residual_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t cols,
+                                                                 int has_post_weight,
+                                                                 int64_t gate_groups);
+CF_API int cf_gated_residual_rmsnorm_backward(
+    const void *d_normalised, const void *d_residual_out, const void *x, const void *residual,
+    const void *weight, const void *post_weight, const void *gate, int64_t gate_groups,
+    int weight_dtype, const float *stats, void *dx, void *d_residual, void *d_weight,
+    void *d_post_weight, void *d_gate, int64_t rows, int64_t cols, float residual_scale, int dtype,
+    void *workspace, size_t workspace_bytes, cf_stream_t stream);
+
 /* Allocation-free form of cf_lora_linear, for callers that cannot allocate the
  * workspace: hosts whose device memory is reserved up front by another
  * allocator, foreign-language hosts without a CUDA allocator, and loops that

@@ -1,0 +1,72 @@
+"""Refusals of the feed-forward block's operators that need no GPU: the Python wrappers'
+messages and the C entry points' argument checks, which all return before any CUDA call."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import cuda_force_b200 as cf
+from cuda_force_b200 import _abi
+
+F = ctypes.c_void_p(0x1000)
+BF16, F16, F32 = _abi.CF_DTYPE_BF16, _abi.CF_DTYPE_F16, _abi.CF_DTYPE_F32
+
+
+def test_gated_residual_rmsnorm_refuses():
+    x, w = torch.zeros(2, 3, 8), torch.ones(8)
+    call = cf.gated_residual_rmsnorm
+    with pytest.raises(ValueError, match="same shape"):
+        call(x, torch.zeros(2, 3, 9), w)
+    with pytest.raises(ValueError, match="share one dtype"):
+        call(x, x.half(), w)
+    with pytest.raises(ValueError, match="share one dtype"):
+        call(x.double(), x.double(), w)
+    with pytest.raises(ValueError, match="^weight must be 1-D of length 8"):
+        call(x, x, torch.ones(9))
+    with pytest.raises(ValueError, match="post_weight must be 1-D of length 8"):
+        call(x, x, w, torch.ones(1, 8))
+    for bad in ((9,), (1, 3, 8), (3, 8), (2, 1, 1), (2, 2, 8)):
+        with pytest.raises(ValueError, match="gate must be"):
+            call(x, x, w, None, torch.ones(bad))
+    for fine in ((8,), (1, 1, 8), (2, 1, 8), (2, 3, 8)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(x, x, w, None, torch.ones(fine))
+
+
+def test_gated_residual_rmsnorm_entry_points_refuse():
+    lib = _abi.load()
+
+    def fwd(rows=4, cols=64, groups=1, gate=F, x=F, dt=BF16, wdt=BF16):
+        return lib.cf_gated_residual_rmsnorm(x, F, F, F, gate, groups, wdt, F, F, None, rows, cols,
+                                             1.0, 1e-6, dt, None)
+
+    assert fwd(rows=-1) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(cols=-1) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(groups=0) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(groups=3) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(x=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(dt=7) == _abi.CF_ERR_UNSUPPORTED
+    assert fwd(wdt=F16) == _abi.CF_ERR_UNSUPPORTED
+    assert fwd(rows=1 << 32) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(rows=0) == _abi.CF_OK
+    assert fwd(cols=0) == _abi.CF_OK
+
+    size = lib.cf_gated_residual_rmsnorm_backward_workspace_bytes
+    assert size(0, 64, 1, 0) == 0 and size(4, 64, 1, 3) == 0
+    assert size(1 << 20, 4096, 1, 1) < 1 << 28
+
+    def bwd(rows=4, post=F, dpost=F, gate=F, dgate=F, stats=F, ws=F, ws_bytes=1 << 30):
+        return lib.cf_gated_residual_rmsnorm_backward(
+            F, F, F, F, F, post, gate, 1, BF16, stats, F, F, F, dpost, dgate, rows, 64, 1.0, BF16,
+            ws, ws_bytes, None)
+
+    assert bwd(dpost=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert bwd(gate=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert bwd(stats=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert bwd(ws=None) == _abi.CF_ERR_WORKSPACE
+    assert bwd(ws_bytes=16) == _abi.CF_ERR_WORKSPACE
+    assert bwd(ws=ctypes.c_void_p(0x1008)) == _abi.CF_ERR_MISALIGNED
+    assert bwd(rows=0) == _abi.CF_OK
