@@ -91,7 +91,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _int, _p],
     ),
     "cf_gated_residual_rmsnorm_backward_workspace_bytes": (
-        ctypes.c_size_t, [_i64, _i64, _int, _i64]),
+        ctypes.c_size_t, [_i64, _i64, _int, _i64, _int]),
     "cf_gated_residual_rmsnorm_backward": (
         _int,
         [_p, _p, _p, _p, _p, _p, _p, _i64, _int, _p, _p, _p, _p, _p, _p, _i64, _i64,

@@ -18,10 +18,17 @@
 // HBM-bound: forward reads x and residual and writes n and h, backward reads x,
 // residual, dn and dh and writes dx and d residual; q and t are kept from the
 // forward pass (8 bytes a row), h is recomputed rather than read back rounded.
-// One row per group of kTpr threads, kPer elements of it in each thread's
-// registers through all passes, so nothing is read twice. Rows beyond the
-// register form (forward 16384 16-bit or 8192 fp32 elements, backward 8192)
-// take looping kernels that read their row again.
+//
+// Each row needs two sums over the row, the second of values that the first
+// scales, so a kernel that loads a row, reduces, and loads the next leaves the
+// memory idle unless other rows are in flight. Forward has one row for each
+// group of kTpr threads and enough CTAs on an SM. Backward holds the parameters'
+// sums in registers, so few CTAs fit; they are persistent and stream their rows
+// through a ring in shared memory filled by bulk copies, so the next rows arrive
+// while this one is reduced. Rows that are not whole 16-byte units, or not
+// aligned to them, take the same passes element by element (simple kernels);
+// rows longer than 16384 16-bit or 8192 fp32 elements (backward: 8192) take
+// looping kernels that read their row again.
 //
 // The parameters' gradients are sums over rows. Each backward CTA walks a
 // fixed range of rows ("slot") and keeps its sums in registers; slots are
@@ -31,8 +38,10 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cf_common.cuh"
+#include "ptx.cuh"
 
 namespace cfb {
 namespace {
@@ -67,18 +76,17 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
 
 // How a row is spread over threads: chunk i of thread t starts at column
 // (i * kTpr + t) * kVec, so a warp's accesses are contiguous.
-// Backward holds four values and up to three sums for each element: 8 of them
-// are about 80 registers, 16 spill at 512 threads and more.
-constexpr int kBackwardPer = 8;
-template <typename T>
-constexpr int kForwardPer = sizeof(T) == 4 ? 8 : 16;
-
-template <typename T, bool kWide, int kElems>
+template <int kElems, int kPerAccess>
 struct Spread {
-  static constexpr int kPer = kElems;                              // elements per thread
-  static constexpr int kVec = kWide ? 16 / static_cast<int>(sizeof(T)) : 1;  // per access
+  static constexpr int kPer = kElems;        // elements per thread
+  static constexpr int kVec = kPerAccess;    // elements per access
   static constexpr int kChunks = kPer / kVec;
 };
+// Rows of 16-byte units: 16 elements a thread, 8 of fp32.
+template <typename T>
+using Wide = Spread<sizeof(T) == 4 ? 8 : 16, 16 / static_cast<int>(sizeof(T))>;
+// The simple kernels hold four values and three sums of each element.
+using Simple = Spread<8, 1>;
 
 template <typename T, int kVec>
 __device__ __forceinline__ void load_vec(const T *p, float *f) {
@@ -93,6 +101,89 @@ __device__ __forceinline__ void store_vec(T *p, const float *f) {
 #pragma unroll
   for (int e = 0; e < kVec; ++e) v.v[e] = from_float<T>(f[e]);
   *reinterpret_cast<Pack<T, kVec> *>(p) = v;
+}
+
+// The kernels for rows of 16-byte units work on pairs of floats with packed arithmetic: at 16 bits
+// an element these kernels are otherwise bound by instruction issue (84
+// instructions an element backward, 36 forward, before this; see the kernels).
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) { return {ptx::pack_f32x2(lo, hi)}; }
+__device__ __forceinline__ Pair both(float v) { return {ptx::splat_f32x2(v)}; }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) { return {ptx::mul_f32x2(a.v, b.v)}; }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) { return {ptx::add_f32x2(a.v, b.v)}; }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  return {ptx::fma_f32x2(a.v, b.v, c.v)};
+}
+__device__ __forceinline__ float sum(Pair a) {
+  const float2 f = ptx::unpack_f32x2(a.v);
+  return f.x + f.y;
+}
+
+// 16 bytes of T as pairs.
+template <typename T>
+__device__ __forceinline__ Pair widen(uint32_t two);
+template <>
+__device__ __forceinline__ Pair widen<__nv_bfloat16>(uint32_t two) {
+  return pair(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ Pair widen<__half>(uint32_t two) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&two));
+  return pair(f.x, f.y);
+}
+
+template <typename T, int kPairs>
+__device__ __forceinline__ void widen(const uint4 &v, Pair (&f)[kPairs]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    f[0] = widen<T>(v.x);
+    f[1] = widen<T>(v.y);
+    f[2] = widen<T>(v.z);
+    f[3] = widen<T>(v.w);
+  }
+}
+
+// kVec elements (16 bytes of 16-bit elements, or any whole number of float4s).
+template <typename T, int kVec>
+__device__ __forceinline__ void load_pairs(const T *p, Pair (&f)[kVec / 2]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kVec / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4 *>(p)[i];
+      f[2 * i] = pair(v.x, v.y);
+      f[2 * i + 1] = pair(v.z, v.w);
+    }
+  } else {
+    static_assert(kVec == 8, "one 16-byte access");
+    widen<T>(*reinterpret_cast<const uint4 *>(p), f);
+  }
+}
+
+template <typename T, int kVec>
+__device__ __forceinline__ void store_pairs(T *p, const Pair (&f)[kVec / 2]) {
+  float2 v[kVec / 2];
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) v[i] = ptx::unpack_f32x2(f[i].v);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kVec / 4; ++i) {
+      reinterpret_cast<float4 *>(p)[i] =
+          make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
+    }
+  } else {
+    static_assert(kVec == 8, "one 16-byte access");
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = std::is_same_v<T, __half> ? ptx::pack_f16x2(v[i].x, v[i].y)
+                                       : ptx::pack_bf16x2(v[i].x, v[i].y);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // Sum over the kTpr threads of a row. Groups of one warp need no barrier;
@@ -130,6 +221,9 @@ struct NormArgs {
   float *means; // [rows][2]: m1 and m2 (long rows)
   int64_t slots, group_chunks, rows_per_slot;
   bool whole_groups;  // a slot holds whole gate groups and writes their gradients itself
+  // staged kernels
+  int stages;
+  unsigned *err;
 };
 
 constexpr int kThreadsSmall = 128;  // CTA of the warp-per-row form: four rows
@@ -139,10 +233,104 @@ constexpr int cta_threads() { return kTpr == kWarp ? kThreadsSmall : kTpr; }
 
 // ---------------------------------------------------------------- forward
 
-template <typename T, typename TW, int kTpr, bool kWide>
-__global__ void __launch_bounds__(cta_threads<kTpr>())
+// One row for each group of threads, in registers through both passes. The
+// hardware hides one row's two sums behind other CTAs' rows: 58 us at [8192,
+// 4096] bf16 with scalar arithmetic, against 73 us for persistent CTAs with the
+// backward kernel's ring and staged weights.
+template <typename T, typename TW, int kTpr>
+__global__ void __launch_bounds__(cta_threads<kTpr>(), 1536 / cta_threads<kTpr>())
     gated_norm_kernel(const NormArgs a) {
-  using S = Spread<T, kWide, kForwardPer<T>>;
+  using S = Wide<T>;
+  constexpr int kPairs = S::kVec / 2;
+  __shared__ float buf[2][32];
+  int parity = 0;
+  constexpr int kRows = cta_threads<kTpr>() / kTpr;
+  const int t = threadIdx.x % kTpr;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTpr;
+  if (row >= a.rows) return;  // whole warps, and only where a row is one warp
+  const int cols = static_cast<int>(a.cols);
+  const float inv_cols = 1.0f / static_cast<float>(cols);
+  const T *x = static_cast<const T *>(a.x) + row * a.cols;
+  const T *r = static_cast<const T *>(a.residual) + row * a.cols;
+  const TW *weight = static_cast<const TW *>(a.weight);
+  const TW *post = static_cast<const TW *>(a.post);
+  const TW *gate = a.gate ? static_cast<const TW *>(a.gate) + row / a.gate_rows * a.cols : nullptr;
+  // The inputs stay packed until they are used: more CTAs fit on an SM.
+  uint4 xr[S::kChunks], rr[S::kChunks];
+  Pair h[S::kChunks][kPairs], ss = both(0.0f);
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      xr[i] = *reinterpret_cast<const uint4 *>(x + c);
+      rr[i] = *reinterpret_cast<const uint4 *>(r + c);
+    }
+  }
+  float q = 1.0f;
+  if (post != nullptr) {
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      if ((i * kTpr + t) * S::kVec < cols) {
+        Pair p[kPairs];
+        widen<T>(xr[i], p);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) ss = fma(p[e], p[e], ss);
+      }
+    }
+    q = rsqrtf(row_sum<kTpr>(sum(ss), buf, parity) * inv_cols + a.eps);
+    ss = both(0.0f);
+  }
+  const Pair q2 = both(q), scale2 = both(a.scale);
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      Pair p[kPairs], w[kPairs];
+      widen<T>(xr[i], p);
+      widen<T>(rr[i], h[i]);
+      if (post != nullptr) {
+        load_pairs<TW, S::kVec>(post + c, w);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) p[e] = p[e] * q2 * w[e];
+      }
+      if (gate != nullptr) {
+        load_pairs<TW, S::kVec>(gate + c, w);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) p[e] = p[e] * w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) {
+        h[i][e] = fma(scale2, h[i][e], p[e]);
+        ss = fma(h[i][e], h[i][e], ss);
+      }
+      store_pairs<T, S::kVec>(static_cast<T *>(a.h) + row * a.cols + c, h[i]);
+    }
+  }
+  const float rt = rsqrtf(row_sum<kTpr>(sum(ss), buf, parity) * inv_cols + a.eps);
+  const Pair rt2 = both(rt);
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      Pair w[kPairs];
+      load_pairs<TW, S::kVec>(weight + c, w);
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) w[e] = h[i][e] * rt2 * w[e];
+      store_pairs<T, S::kVec>(static_cast<T *>(a.n) + row * a.cols + c, w);
+    }
+  }
+  if (a.stats != nullptr && t == 0) {
+    a.stats[2 * row] = q;
+    a.stats[2 * row + 1] = rt;
+  }
+}
+
+// The same passes with the row in registers, element by element, one row for
+// each group of threads.
+template <typename T, typename TW, int kTpr>
+__global__ void __launch_bounds__(cta_threads<kTpr>())
+    gated_norm_simple_kernel(const NormArgs a) {
+  using S = Simple;
   __shared__ float buf[2][32];
   int parity = 0;
   constexpr int kRows = cta_threads<kTpr>() / kTpr;
@@ -285,12 +473,318 @@ __device__ __forceinline__ void slot_rows(const NormArgs &a, int64_t slot, int64
   }
 }
 
+// CTAs of the backward kernel on an SM: 512 threads at up to 128 registers (one
+// CTA of 1024 threads has 64).
+template <int kTpr>
+constexpr int backward_ctas() {
+  return cta_threads<kTpr>() > 512 ? 1 : 512 / cta_threads<kTpr>();
+}
+
+// ---------------------------------------------------------------- row ring
+
+constexpr int kMaxStages = 4;
+
+// The ring of one group of kTpr threads: each stage holds a row of up to
+// kArrays inputs. Thread 0 of the group issues the copies; every thread waits.
+// A wait that runs out records the error and stops all later waits and copies
+// of the thread, and the kernel runs to its end on what is there.
+template <int kArrays>
+struct RowRing {
+  const uint8_t *src[kArrays];  // null: not read
+  uint8_t *smem;
+  uint64_t *full;
+  unsigned *err;
+  uint32_t row_bytes;
+  int stages, stage = 0;
+  uint32_t phase = 0, outstanding = 0;
+  bool failed = false;
+
+  __device__ __forceinline__ void init() {
+    for (int s = 0; s < stages; ++s) ptx::mbar_init(&full[s], 1);
+    ptx::fence_mbar_init();
+  }
+
+  __device__ __forceinline__ void issue(int to, int64_t row) {
+    if (failed) return;
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) bytes += src[i] ? row_bytes : 0;
+    ptx::mbar_expect_tx(&full[to], bytes);
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) {
+      if (src[i]) {
+        ptx::bulk_load(smem + (to * kArrays + i) * row_bytes, src[i] + row * row_bytes, row_bytes,
+                       &full[to]);
+      }
+    }
+    outstanding |= 1u << to;
+  }
+
+  // Waits for the current stage.
+  __device__ __forceinline__ void wait() {
+    if (!failed && !ptx::mbar_wait(&full[stage], phase)) {
+      atomicOr(err, kDevErrTimeout);
+      failed = true;
+    }
+    if (!failed) outstanding &= ~(1u << stage);
+  }
+
+  template <typename T>
+  __device__ __forceinline__ const T *row(int array) const {
+    return reinterpret_cast<const T *>(smem + (stage * kArrays + array) * row_bytes);
+  }
+
+  __device__ __forceinline__ void advance() {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+
+  // After a failed wait: lets copies in flight land before the CTA's shared
+  // memory goes away (bounded).
+  __device__ __forceinline__ void drain() {
+    if (!failed) return;
+    for (int s = 0; s < stages; ++s) {
+      if (outstanding & (1u << s)) {
+        ptx::mbar_wait(&full[s], s < stage ? phase ^ 1 : phase, 200000000ull);
+      }
+    }
+  }
+};
+
+// All threads of a row's group.
+template <int kTpr>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (kTpr > kWarp) {
+    __syncthreads();
+  } else {
+    __syncwarp();
+  }
+}
+
+// weight and post_weight (ones without it) as fp32 in shared memory, loaded once
+// by a persistent CTA. A thread reads kVec consecutive values as float4s; they
+// are stored so that each of its float4s is next to its neighbours' (kVec 8: the
+// first halves of all groups of eight, then the second halves), which keeps the
+// accesses free of bank conflicts.
+template <int kVec>
+__device__ __forceinline__ int staged_at(int c, int cols) {
+  return kVec == 8 ? (c & 4 ? cols / 2 : 0) + (c >> 3) * 4 + (c & 3) : c;
+}
+
+template <typename TW, int kVec>
+__device__ __forceinline__ void stage_weights(float *post_s, float *weight_s, const void *post,
+                                              const void *weight, int cols) {
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    const int at = staged_at<kVec>(c, cols);
+    weight_s[at] = to_float<TW>(static_cast<const TW *>(weight)[c]);
+    post_s[at] = post ? to_float<TW>(static_cast<const TW *>(post)[c]) : 1.0f;
+  }
+}
+
+template <int kVec>
+__device__ __forceinline__ void load_staged(const float *w, int c, int cols,
+                                            Pair (&f)[kVec / 2]) {
+#pragma unroll
+  for (int i = 0; i < kVec / 4; ++i) {
+    const float4 v = *reinterpret_cast<const float4 *>(w + staged_at<kVec>(c + 4 * i, cols));
+    f[2 * i] = pair(v.x, v.y);
+    f[2 * i + 1] = pair(v.z, v.w);
+  }
+}
+
 // kShared: a row of the gate serves gate_rows > 1 rows, so its gradient is a
 // sum; otherwise there is none, or one for each row.
-template <typename T, typename TW, int kTpr, bool kWide, bool kShared>
-__global__ void __launch_bounds__(cta_threads<kTpr>())
+template <typename T, typename TW, int kTpr, bool kShared>
+__global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
     gated_norm_backward_kernel(const NormArgs a) {
-  using S = Spread<T, kWide, kBackwardPer>;
+  using S = Wide<T>;
+  constexpr int kPairs = S::kVec / 2;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  constexpr int kSlots = cta_threads<kTpr>() / kTpr;
+  __shared__ float buf[2][32];
+  __shared__ __align__(8) uint64_t full[kSlots][kMaxStages];
+  int parity = 0;
+  const int in_cta = threadIdx.x / kTpr;
+  const int t = threadIdx.x % kTpr;
+  const int64_t slot = static_cast<int64_t>(blockIdx.x) * kSlots + in_cta;
+  const int cols = static_cast<int>(a.cols);
+  const float inv_cols = 1.0f / static_cast<float>(cols);
+  float *post_s = reinterpret_cast<float *>(smem_raw);
+  float *weight_s = post_s + cols;
+  int64_t begin = 0, end = 0;
+  if (slot < a.slots) slot_rows(a, slot, kShared ? a.gate_rows : a.rows, begin, end);
+
+  RowRing<4> ring;
+  ring.src[0] = static_cast<const uint8_t *>(a.x);
+  ring.src[1] = static_cast<const uint8_t *>(a.residual);
+  ring.src[2] = static_cast<const uint8_t *>(a.dn);
+  ring.src[3] = static_cast<const uint8_t *>(a.dh);
+  ring.row_bytes = static_cast<uint32_t>(cols * sizeof(T));
+  ring.stages = a.stages;
+  ring.smem = smem_raw + 2 * cols * sizeof(float) +
+              static_cast<size_t>(in_cta) * a.stages * 4 * ring.row_bytes;
+  ring.full = full[in_cta];
+  ring.err = a.err;
+  if (t == 0) {
+    ring.init();
+    for (int s = 0; s < a.stages && begin + s < end; ++s) ring.issue(s, begin + s);
+  }
+  stage_weights<TW, S::kVec>(post_s, weight_s, a.post, a.weight, cols);
+  __syncthreads();
+  if (slot >= a.slots) return;  // whole warps, and only where a row is one warp
+
+  Pair sum_w[S::kChunks][kPairs], sum_p[S::kChunks][kPairs], sum_g[S::kChunks][kPairs];
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) sum_w[i][e] = sum_p[i][e] = sum_g[i][e] = both(0.0f);
+  }
+  float2 stats = begin < end ? reinterpret_cast<const float2 *>(a.stats)[begin] : float2{};
+  const Pair scale2 = both(a.scale);
+
+  for (int64_t row = begin; row < end; ++row) {
+    const int64_t base = row * a.cols;
+    const TW *gate = a.gate == nullptr ? nullptr
+                                       : static_cast<const TW *>(a.gate) +
+                                             (kShared ? row / a.gate_rows : row) * a.cols;
+    const Pair q2 = both(stats.x), rt2 = both(stats.y);
+    if (row + 1 < end) stats = reinterpret_cast<const float2 *>(a.stats)[row + 1];
+    ring.wait();
+    const T *x = ring.template row<T>(0);
+    const T *r = ring.template row<T>(1);
+    const T *dn = ring.template row<T>(2);
+    const T *dh = ring.template row<T>(3);
+
+    // hh and a stay in registers for the second pass; d takes a's place there.
+    Pair hh[S::kChunks][kPairs], av[S::kChunks][kPairs];
+    Pair neg_m1 = both(0.0f);
+    if (a.dn != nullptr) {
+      Pair s1 = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < S::kChunks; ++i) {
+        const int c = (i * kTpr + t) * S::kVec;
+        if (c < cols) {
+          Pair p[kPairs], w[kPairs];
+          load_pairs<T, S::kVec>(x + c, p);
+          load_pairs<T, S::kVec>(r + c, hh[i]);
+          load_staged<S::kVec>(post_s, c, cols, w);
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) p[e] = p[e] * q2 * w[e];
+          if (gate != nullptr) {
+            load_pairs<TW, S::kVec>(gate + c, w);
+#pragma unroll
+            for (int e = 0; e < kPairs; ++e) p[e] = p[e] * w[e];
+          }
+          load_staged<S::kVec>(weight_s, c, cols, w);
+          load_pairs<T, S::kVec>(dn + c, av[i]);
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) {
+            hh[i][e] = fma(scale2, hh[i][e], p[e]) * rt2;
+            sum_w[i][e] = fma(av[i][e], hh[i][e], sum_w[i][e]);
+            av[i][e] = av[i][e] * w[e];
+            s1 = fma(av[i][e], hh[i][e], s1);
+          }
+        }
+      }
+      neg_m1 = both(-row_sum<kTpr>(sum(s1), buf, parity) * inv_cols);
+    }
+
+    Pair s2 = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      if (c < cols) {
+        Pair xh[kPairs], w[kPairs], out[kPairs], *d = av[i];
+        if (a.dh != nullptr) {
+          load_pairs<T, S::kVec>(dh + c, out);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) out[e] = both(0.0f);
+        }
+        load_pairs<T, S::kVec>(x + c, xh);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          xh[e] = xh[e] * q2;
+          d[e] = a.dn != nullptr ? fma(rt2, fma(hh[i][e], neg_m1, d[e]), out[e]) : out[e];
+          out[e] = d[e] * scale2;
+        }
+        store_pairs<T, S::kVec>(static_cast<T *>(a.dres) + base + c, out);
+        Pair pw[kPairs];
+        load_staged<S::kVec>(post_s, c, cols, pw);
+        if (gate != nullptr) {
+          load_pairs<TW, S::kVec>(gate + c, w);
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) {
+            out[e] = d[e] * (xh[e] * pw[e]);
+            if constexpr (kShared) sum_g[i][e] = sum_g[i][e] + out[e];
+            d[e] = d[e] * w[e];
+          }
+          if constexpr (!kShared) {
+            store_pairs<TW, S::kVec>(static_cast<TW *>(a.dgate) + base + c, out);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          sum_p[i][e] = fma(d[e], xh[e], sum_p[i][e]);
+          d[e] = d[e] * pw[e];
+          s2 = fma(d[e], xh[e], s2);
+        }
+      }
+    }
+    // Without post_weight there is no first norm: dx = d.
+    Pair neg_m2 = both(0.0f);
+    if (a.post != nullptr) neg_m2 = both(-row_sum<kTpr>(sum(s2), buf, parity) * inv_cols);
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      const int c = (i * kTpr + t) * S::kVec;
+      if (c < cols) {
+        Pair xh[kPairs];
+        load_pairs<T, S::kVec>(x + c, xh);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) xh[e] = fma(xh[e] * q2, neg_m2, av[i][e]) * q2;
+        store_pairs<T, S::kVec>(static_cast<T *>(a.dx) + base + c, xh);
+      }
+    }
+    // The row has been read: its stage takes the row `stages` ahead.
+    group_sync<kTpr>();
+    if (t == 0 && row + a.stages < end) ring.issue(ring.stage, row + a.stages);
+    ring.advance();
+    if constexpr (kShared) {
+      if (a.whole_groups && (row + 1) % a.gate_rows == 0) {
+#pragma unroll
+        for (int i = 0; i < S::kChunks; ++i) {
+          const int c = (i * kTpr + t) * S::kVec;
+          if (c < cols) {
+            store_pairs<TW, S::kVec>(
+                static_cast<TW *>(a.dgate) + row / a.gate_rows * a.cols + c, sum_g[i]);
+          }
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) sum_g[i][e] = both(0.0f);
+        }
+      }
+    }
+  }
+  if (t == 0) ring.drain();
+  const int64_t plane = a.slots * a.cols;
+  float *part = a.part + slot * a.cols;
+#pragma unroll
+  for (int i = 0; i < S::kChunks; ++i) {
+    const int c = (i * kTpr + t) * S::kVec;
+    if (c < cols) {
+      store_pairs<float, S::kVec>(part + c, sum_w[i]);
+      if (a.post) store_pairs<float, S::kVec>(part + plane + c, sum_p[i]);
+      if (kShared && !a.whole_groups) store_pairs<float, S::kVec>(part + 2 * plane + c, sum_g[i]);
+    }
+  }
+}
+
+// The same with the row in registers, element by element.
+template <typename T, typename TW, int kTpr, bool kShared>
+__global__ void __launch_bounds__(cta_threads<kTpr>())
+    gated_norm_backward_simple_kernel(const NormArgs a) {
+  using S = Simple;
   __shared__ float buf[2][32];
   int parity = 0;
   constexpr int kSlots = cta_threads<kTpr>() / kTpr;
@@ -321,17 +815,13 @@ __global__ void __launch_bounds__(cta_threads<kTpr>())
     for (int i = 0; i < S::kChunks; ++i) {
       const int c = (i * kTpr + t) * S::kVec;
       const int o = i * S::kVec;
+#pragma unroll
+      for (int e = 0; e < S::kVec; ++e) xh[o + e] = hh[o + e] = av[o + e] = dv[o + e] = 0.0f;
       if (c < cols) {
         load_vec<T, S::kVec>(static_cast<const T *>(a.x) + base + c, xh + o);
         load_vec<T, S::kVec>(static_cast<const T *>(a.residual) + base + c, hh + o);
         if (a.dn) load_vec<T, S::kVec>(static_cast<const T *>(a.dn) + base + c, av + o);
         if (a.dh) load_vec<T, S::kVec>(static_cast<const T *>(a.dh) + base + c, dv + o);
-      }
-#pragma unroll
-      for (int e = 0; e < S::kVec; ++e) {
-        if (c >= cols) xh[o + e] = hh[o + e] = 0.0f;
-        if (c >= cols || !a.dn) av[o + e] = 0.0f;
-        if (c >= cols || !a.dh) dv[o + e] = 0.0f;
       }
     }
 #pragma unroll
@@ -431,15 +921,12 @@ __global__ void __launch_bounds__(cta_threads<kTpr>())
   const int64_t plane = a.slots * a.cols;
   float *part = a.part + slot * a.cols;
 #pragma unroll
-  for (int i = 0; i < S::kChunks; ++i) {
-    const int c = (i * kTpr + t) * S::kVec;
-#pragma unroll
-    for (int e = 0; e < S::kVec; ++e) {
-      if (c + e < cols) {
-        part[c + e] = sum_w[i * S::kVec + e];
-        if (post != nullptr) part[plane + c + e] = sum_p[i * S::kVec + e];
-        if (kShared && !a.whole_groups) part[2 * plane + c + e] = sum_g[i * S::kVec + e];
-      }
+  for (int i = 0; i < S::kPer; ++i) {
+    const int c = i * kTpr + t;
+    if (c < cols) {
+      part[c] = sum_w[i];
+      if (post != nullptr) part[plane + c] = sum_p[i];
+      if (kShared && !a.whole_groups) part[2 * plane + c] = sum_g[i];
     }
   }
 }
@@ -538,7 +1025,7 @@ __global__ void __launch_bounds__(kColumnThreads)
 
 // Adds the slots' partial sums. blockIdx.y: 0 weight, 1 post_weight, 2 + g the
 // gate's group g. A thread adds every kFinishRows-th slot, in order.
-constexpr int kFinishCols = 32, kFinishRows = 16;
+constexpr int kFinishCols = 32, kFinishRows = 32;
 
 template <typename TW>
 __global__ void __launch_bounds__(kFinishCols *kFinishRows)
@@ -554,7 +1041,7 @@ __global__ void __launch_bounds__(kFinishCols *kFinishRows)
   const float *src = part + (min(which, int64_t{2}) * slots + first) * cols + c;
   float s = 0.0f;
   if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t k = threadIdx.y; k < count; k += kFinishRows) s += src[k * cols];
   }
   sums[threadIdx.y][threadIdx.x] = s;
@@ -578,11 +1065,15 @@ int threads_per_row(int64_t cols, int per) {
 }
 
 
-// The backward pass's slots: about as many rows at a time as an SM holds (512
-// threads of them), since more only add partial sums.
-void plan_slots(NormArgs &a, bool shared_gate) {
-  const int tpr = threads_per_row(a.cols, kBackwardPer);
-  const int64_t per_sm = tpr == 0 ? 2 : std::max(1, 512 / tpr);
+// The longest row of the staged and simple backward kernels.
+constexpr int64_t kBackwardMaxCols = 8192;
+
+// The backward pass's slots: as many rows at a time as keep the memory busy (512
+// threads an SM; eight rows of a warp each), since more only add partial sums.
+void plan_slots(NormArgs &a, int dtype, bool shared_gate) {
+  const int tpr =
+      a.cols > kBackwardMaxCols ? 0 : threads_per_row(a.cols, dtype == CF_DTYPE_F32 ? 8 : 16);
+  const int64_t per_sm = tpr == 0 ? 2 : tpr == kWarp ? 8 : std::max(1, 512 / tpr);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.rows, per_sm * sm_count()));
   const int64_t group_rows = shared_gate ? a.gate_rows : a.rows;
   const int64_t groups = a.rows / group_rows;
@@ -607,21 +1098,44 @@ size_t part_bytes(const NormArgs &a, bool post, bool shared_gate) {
   return (bytes + 255) & ~static_cast<size_t>(255);
 }
 
+// Stages of a ring whose CTA holds `groups` of them beside its two fp32 weight
+// rows, with `ctas` such CTAs on an SM: as many as fit, up to kMaxStages.
+constexpr int64_t kRingSmem = int64_t{216} << 10;  // an SM has 227 KB for CTAs
+int ring_stages(int arrays, int64_t cols, int64_t elem, int groups, int ctas) {
+  const int64_t left = kRingSmem / ctas - 2 * cols * 4;
+  return static_cast<int>(
+      std::min<int64_t>(kMaxStages, std::max<int64_t>(0, left) / (arrays * cols * elem * groups)));
+}
+
+template <auto Kernel>
+int launch_staged(NormArgs a, int arrays, int64_t elem, int groups, unsigned grid, int threads,
+                  int ctas, cudaStream_t s) {
+  while (ctas > 1 && ring_stages(arrays, a.cols, elem, groups, ctas) < 2) ctas /= 2;
+  a.stages = ring_stages(arrays, a.cols, elem, groups, ctas);
+  if (a.stages < 1) return CF_ERR_UNSUPPORTED;  // not for any length the kernels are built for
+  a.err = device_error_word();
+  if (a.err == nullptr) return record_cuda_error(cudaGetLastError());
+  const size_t smem = 2 * a.cols * 4 + static_cast<size_t>(a.stages) * arrays * a.cols * elem * groups;
+  if (int st = allow_dynamic_smem<Kernel>(kRingSmem)) return st;
+  Kernel<<<grid, threads, smem, s>>>(a);
+  return check_launch();
+}
+
 template <typename T, typename TW, int kTpr>
 int launch_forward(const NormArgs &a, bool wide, cudaStream_t s) {
   constexpr int kRows = cta_threads<kTpr>() / kTpr;
   const unsigned grid = static_cast<unsigned>((a.rows + kRows - 1) / kRows);
   if (wide) {
-    gated_norm_kernel<T, TW, kTpr, true><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
+    gated_norm_kernel<T, TW, kTpr><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
   } else {
-    gated_norm_kernel<T, TW, kTpr, false><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
+    gated_norm_simple_kernel<T, TW, kTpr><<<grid, cta_threads<kTpr>(), 0, s>>>(a);
   }
   return check_launch();
 }
 
 template <typename T, typename TW>
 int forward(const NormArgs &a, bool wide, cudaStream_t s) {
-  switch (threads_per_row(a.cols, kForwardPer<T>)) {
+  switch (threads_per_row(a.cols, wide ? Wide<T>::kPer : Simple::kPer)) {
     case 32: return launch_forward<T, TW, 32>(a, wide, s);
     case 128: return launch_forward<T, TW, 128>(a, wide, s);
     case 256: return launch_forward<T, TW, 256>(a, wide, s);
@@ -634,27 +1148,39 @@ int forward(const NormArgs &a, bool wide, cudaStream_t s) {
   }
 }
 
-template <typename T, typename TW, int kTpr, bool kWide>
-int launch_backward(const NormArgs &a, cudaStream_t s) {
-  constexpr int kSlots = cta_threads<kTpr>() / kTpr;
-  const unsigned grid = static_cast<unsigned>((a.slots + kSlots - 1) / kSlots);
+template <typename T, typename TW, int kTpr>
+int launch_backward(const NormArgs &a, bool wide, cudaStream_t s) {
   constexpr int kThreads = cta_threads<kTpr>();
-  if (a.gate != nullptr && a.gate_rows > 1) {
-    gated_norm_backward_kernel<T, TW, kTpr, kWide, true><<<grid, kThreads, 0, s>>>(a);
-  } else {
-    gated_norm_backward_kernel<T, TW, kTpr, kWide, false><<<grid, kThreads, 0, s>>>(a);
+  constexpr int kSlots = kThreads / kTpr;
+  const unsigned grid = static_cast<unsigned>((a.slots + kSlots - 1) / kSlots);
+  const bool shared = a.gate != nullptr && a.gate_rows > 1;
+  if (!wide) {
+    if (shared) {
+      gated_norm_backward_simple_kernel<T, TW, kTpr, true><<<grid, kThreads, 0, s>>>(a);
+    } else {
+      gated_norm_backward_simple_kernel<T, TW, kTpr, false><<<grid, kThreads, 0, s>>>(a);
+    }
+    return check_launch();
   }
-  return check_launch();
+  // The staged kernel's widest group covers kBackwardMaxCols.
+  constexpr int kWideTpr =
+      std::min<int>(kTpr, static_cast<int>(kBackwardMaxCols / Wide<T>::kPer));
+  constexpr int ctas = backward_ctas<kWideTpr>();
+  return shared ? launch_staged<gated_norm_backward_kernel<T, TW, kWideTpr, true>>(
+                      a, 4, sizeof(T), kSlots, grid, kThreads, ctas, s)
+                : launch_staged<gated_norm_backward_kernel<T, TW, kWideTpr, false>>(
+                      a, 4, sizeof(T), kSlots, grid, kThreads, ctas, s);
 }
 
 template <typename T, typename TW>
 int backward(const NormArgs &a, bool wide, void *dweight, void *dpost, cudaStream_t s) {
   int st = CF_OK;
-  switch (threads_per_row(a.cols, kBackwardPer)) {
-#define CFB_CASE(tpr)                                                  \
-  case tpr:                                                            \
-    st = wide ? launch_backward<T, TW, tpr, true>(a, s)                \
-              : launch_backward<T, TW, tpr, false>(a, s);              \
+  switch (a.cols > kBackwardMaxCols
+              ? 0
+              : threads_per_row(a.cols, wide ? Wide<T>::kPer : Simple::kPer)) {
+#define CFB_CASE(tpr)                              \
+  case tpr:                                        \
+    st = launch_backward<T, TW, tpr>(a, wide, s);  \
     break
     CFB_CASE(32);
     CFB_CASE(128);
@@ -767,16 +1293,16 @@ int cf_gated_residual_rmsnorm(const void *x, const void *residual, const void *w
 
 size_t cf_gated_residual_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t cols,
                                                           int has_post_weight,
-                                                          int64_t gate_groups) {
+                                                          int64_t gate_groups, int dtype) {
   if (rows <= 0 || cols <= 0 || (gate_groups > 0 && rows % gate_groups != 0)) return 0;
   cfb::NormArgs a{};
   a.rows = rows;
   a.cols = cols;
   const bool shared = gate_groups > 0 && gate_groups < rows;
   a.gate_rows = gate_groups > 0 ? rows / gate_groups : rows;
-  cfb::plan_slots(a, shared);
+  cfb::plan_slots(a, dtype, shared);
   size_t bytes = cfb::part_bytes(a, has_post_weight != 0, shared);
-  if (cfb::threads_per_row(cols, cfb::kBackwardPer) == 0) {
+  if (cols > cfb::kBackwardMaxCols) {
     bytes += static_cast<size_t>(rows) * 2 * sizeof(float);
   }
   return bytes;
@@ -815,9 +1341,9 @@ int cf_gated_residual_rmsnorm_backward(
   a.dres = d_residual;
   a.dgate = d_gate;
   const bool shared = gate != nullptr && a.gate_rows > 1;
-  cfb::plan_slots(a, shared);
+  cfb::plan_slots(a, dtype, shared);
   const size_t need = cf_gated_residual_rmsnorm_backward_workspace_bytes(
-      rows, cols, post_weight != nullptr, gate ? gate_groups : 0);
+      rows, cols, post_weight != nullptr, gate ? gate_groups : 0, dtype);
   if (workspace == nullptr || workspace_bytes < need) return CF_ERR_WORKSPACE;
   if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
   a.part = static_cast<float *>(workspace);

@@ -457,7 +457,7 @@ std::vector<at::Tensor> block_norm_backward(
   if (empty) return typed();
   const int dtype = dtype_code(x, "x");
   const size_t ws_bytes = cf_gated_residual_rmsnorm_backward_workspace_bytes(
-      rows, cols, p.post.defined(), p.gate.defined() ? gate_groups : 0);
+      rows, cols, p.post.defined(), p.gate.defined() ? gate_groups : 0, dtype);
   at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
   check_status(
       cf_gated_residual_rmsnorm_backward(

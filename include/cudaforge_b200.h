@@ -321,7 +321,7 @@ CF_API int cf_gated_residual_rmsnorm(const void *x, const void *residual, const 
  * for no gate) bytes of device memory, 16-byte aligned. rows == 0 writes nothing. */
 CF_API size_t cf_gated_residual_rmsnorm_backward_workspace_bytes(int64_t rows, int64_t cols,
                                                                  int has_post_weight,
-                                                                 int64_t gate_groups);
+                                                                 int64_t gate_groups, int dtype);
 CF_API int cf_gated_residual_rmsnorm_backward(
     const void *d_normalised, const void *d_residual_out, const void *x, const void *residual,
     const void *weight, const void *post_weight, const void *gate, int64_t gate_groups,

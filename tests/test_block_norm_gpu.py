@@ -284,7 +284,7 @@ def test_c_entry_checks_the_workspace(cuda_device):
     x = torch.randn(8, 128, device=cuda_device)
     w = torch.ones(128, device=cuda_device)
     stats = torch.ones(8, 2, device=cuda_device)
-    need = lib.cf_gated_residual_rmsnorm_backward_workspace_bytes(8, 128, 0, 0)
+    need = lib.cf_gated_residual_rmsnorm_backward_workspace_bytes(8, 128, 0, 0, _abi.CF_DTYPE_F32)
     assert need >= 128 * 4
     ws = torch.empty(need, dtype=torch.uint8, device=cuda_device)
     out = [torch.empty_like(x), torch.empty_like(x), torch.empty_like(w)]

@@ -55,8 +55,8 @@ def test_gated_residual_rmsnorm_entry_points_refuse():
     assert fwd(cols=0) == _abi.CF_OK
 
     size = lib.cf_gated_residual_rmsnorm_backward_workspace_bytes
-    assert size(0, 64, 1, 0) == 0 and size(4, 64, 1, 3) == 0
-    assert size(1 << 20, 4096, 1, 1) < 1 << 28
+    assert size(0, 64, 1, 0, BF16) == 0 and size(4, 64, 1, 3, BF16) == 0
+    assert size(1 << 20, 4096, 1, 1, BF16) < 1 << 28
 
     def bwd(rows=4, post=F, dpost=F, gate=F, dgate=F, stats=F, ws=F, ws_bytes=1 << 30):
         return lib.cf_gated_residual_rmsnorm_backward(
