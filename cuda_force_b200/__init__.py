@@ -6,6 +6,7 @@ from __future__ import annotations
 
 from cuda_force_b200.ops import (
     CUDA_KERNELS_AVAILABLE,
+    FP8_BLOCK_SIZE,
     KERNEL_DTYPES,
     QUANT_BLOCK_SIZE,
     backend_report,
@@ -13,12 +14,15 @@ from cuda_force_b200.ops import (
     fused_residual_rmsnorm,
     gated_residual_rmsnorm,
     kernel_supports,
+    linear_fp8,
     lora_linear,
     lora_linear_int8,
     lora_merge_quantize_int8,
     matmul_f32,
+    matmul_fp8,
     quantization_error,
     quantize_dequantize,
+    quantize_fp8,
     quantize_int8,
     quantize_int8_many,
     rmsnorm,
@@ -30,6 +34,7 @@ __version__ = "0.1.0"
 
 __all__ = [
     "CUDA_KERNELS_AVAILABLE",
+    "FP8_BLOCK_SIZE",
     "KERNEL_DTYPES",
     "QUANT_BLOCK_SIZE",
     "__version__",
@@ -38,12 +43,15 @@ __all__ = [
     "fused_residual_rmsnorm",
     "gated_residual_rmsnorm",
     "kernel_supports",
+    "linear_fp8",
     "lora_linear",
     "lora_linear_int8",
     "lora_merge_quantize_int8",
     "matmul_f32",
+    "matmul_fp8",
     "quantization_error",
     "quantize_dequantize",
+    "quantize_fp8",
     "quantize_int8",
     "quantize_int8_many",
     "rmsnorm",

@@ -97,6 +97,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _p, _p, _p, _p, _p, _i64, _int, _p, _p, _p, _p, _p, _p, _i64, _i64,
          ctypes.c_float, _int, _p, ctypes.c_size_t, _p],
     ),
+    "cf_quantize_fp8": (_int, [_p, _int, _p, _p, _i64, _i64, _int, _p]),
+    "cf_matmul_fp8": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
+    "cf_linear_fp8_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "cf_linear_fp8": (
+        _int, [_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, ctypes.c_size_t, _p]),
     "cf_lora_linear_noalloc": (
         _int,
         [_p, _p, _int, _p, _int, _p, _int, _p, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _p],

@@ -1,0 +1,787 @@
+// 8-bit floating-point (e4m3) quantisation with a scale for each block of 128,
+// and the matrix product of operands held that way, for sm_100a.
+//
+//   scale = fl32(absmax / 448), 1 when not > 0 (zero, NaN, underflow)
+//   code  = e4m3(fl32(x / scale)), nearest even, saturating at +-448, NaN kept
+// over blocks of 1 x 128 (activations) or 128 x 128 (weights); the last block of
+// a row may be shorter. The product of a [m, k] in 1 x 128 blocks and b [n, k]
+// in 128 x 128 blocks is
+//   y[m, n] = sum_kb a_scale[m, kb] b_scale[n / 128, kb] (sum_{k in kb} a[m, k] b[n, k])
+// The inner sums are exact products accumulated in fp32 by the tensor core; the
+// outer sum is fp32 in registers: scales are arbitrary fp32 numbers, so they
+// cannot ride on the MMA's own power-of-two block scales.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "cf_common.cuh"
+#include "gemm_common.cuh"
+#include "ptx.cuh"
+
+namespace cfb {
+namespace {
+
+constexpr int kBlock = CF_FP8_BLOCK_SIZE;
+constexpr float kE4m3Max = 448.0f;
+
+// ---------------------------------------------------------------- quantisation
+
+// Scale of a block from the bit pattern of its absmax (a NaN's is the largest).
+__device__ __forceinline__ float fp8_scale(unsigned absmax_bits) {
+  const float s = __fdiv_rn(__uint_as_float(absmax_bits), kE4m3Max);
+  return s > 0.0f ? s : 1.0f;
+}
+
+// Whether x / s may be formed as in fp8_quotient for every element of a block: s
+// far enough from the ends of the range that the residual x - q s is exact for
+// every quotient that does not round to zero, and no infinity or NaN.
+__device__ __forceinline__ bool fp8_fast(unsigned absmax_bits, float s) {
+  return absmax_bits < 0x7f800000u && s >= 0x1p-60f && s <= 0x1p100f;
+}
+
+// fl32(x / s) without a division: r = fl32(1 / s), q0 = fl(x r), the exact
+// residual and Markstein's correction step (as quant_math.cuh).
+__device__ __forceinline__ float fp8_quotient(float x, float s, float r) {
+  const float q0 = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q0, s, x), r, q0);
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Eight elements to eight codes.
+__device__ __forceinline__ uint2 fp8_codes(const float (&f)[8], float s, float r, bool fast) {
+  float q[8];
+  if (fast) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = fp8_quotient(f[i], s, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(f[i], s);
+  }
+  return make_uint2(e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16,
+                    e4m3x2(q[4], q[5]) | e4m3x2(q[6], q[7]) << 16);
+}
+
+__device__ __forceinline__ unsigned absmax_bits(const float (&f)[8]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return m;
+}
+
+template <typename T>
+__device__ __forceinline__ float as_float(T v) {
+  if constexpr (std::is_same_v<T, float>) {
+    return v;
+  } else if constexpr (std::is_same_v<T, __half>) {
+    return __half2float(v);
+  } else {
+    return __bfloat162float(v);
+  }
+}
+
+// Eight consecutive elements from p, `left` of them inside the row (the rest
+// are zeros). kWide: p is on a 16-byte boundary and left is 0 or at least 8.
+template <typename T, bool kWide>
+__device__ __forceinline__ void load8(const T *p, int64_t left, float (&f)[8]) {
+  if constexpr (kWide) {
+    if (left <= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+    } else if constexpr (sizeof(T) == 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+      const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+      f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+      const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = as_float<T>(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < left ? as_float<T>(p[i]) : 0.0f;
+  }
+}
+
+template <bool kWide>
+__device__ __forceinline__ void store8(uint8_t *p, int64_t left, uint2 codes) {
+  if constexpr (kWide) {
+    if (left > 0) *reinterpret_cast<uint2 *>(p) = codes;
+  } else {
+    const uint8_t *b = reinterpret_cast<const uint8_t *>(&codes);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < left) p[i] = b[i];
+    }
+  }
+}
+
+constexpr int kQuantThreads = 256;
+
+// 1 x 128 blocks: 16 lanes a block, eight elements a lane; kUnroll blocks a
+// half-warp, loaded before any is reduced.
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(kQuantThreads)
+    fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks,
+                             int64_t cols, int64_t row_blocks) {
+  constexpr int kUnroll = 4;
+  constexpr int kPerCta = kQuantThreads / 16 * kUnroll;
+  const int lane16 = threadIdx.x & 15;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kPerCta + threadIdx.x / 16;
+  float f[kUnroll][8];
+  int64_t at[kUnroll], left[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t b = first + u * (kQuantThreads / 16);
+    const int64_t row = b / row_blocks;
+    const int64_t c = (b - row * row_blocks) * kBlock + lane16 * 8;
+    at[u] = row * cols + c;
+    left[u] = b < blocks ? cols - c : 0;
+    load8<T, kWide>(x + at[u], left[u], f[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    unsigned m = absmax_bits(f[u]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = fp8_scale(m);
+    store8<kWide>(codes + at[u], left[u], fp8_codes(f[u], s, __frcp_rn(s), fp8_fast(m, s)));
+    const int64_t b = first + u * (kQuantThreads / 16);
+    if (lane16 == 0 && b < blocks) scales[b] = s;
+  }
+}
+
+// 128 x 128 blocks: one CTA each, eight rows of eight elements a thread.
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(kQuantThreads)
+    fp8_quantize_blocks_kernel(const T *x, uint8_t *codes, float *scales, int64_t rows,
+                               int64_t cols) {
+  constexpr int kRowsAtOnce = kQuantThreads / 16;
+  constexpr int kSteps = kBlock / kRowsAtOnce;
+  __shared__ unsigned warp_max[kQuantThreads / kWarp];
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kBlock + (threadIdx.x & 15) * 8;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock + threadIdx.x / 16;
+  float f[kSteps][8];
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int64_t r = r0 + i * kRowsAtOnce;
+    load8<T, kWide>(x + r * cols + c, r < rows ? cols - c : 0, f[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) m = max(m, absmax_bits(f[i]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & (kWarp - 1)) == 0) warp_max[threadIdx.x / kWarp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQuantThreads / kWarp; ++w) m = max(m, warp_max[w]);
+  const float s = fp8_scale(m);
+  const float inv = __frcp_rn(s);
+  const bool fast = fp8_fast(m, s);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int64_t r = r0 + i * kRowsAtOnce;
+    store8<kWide>(codes + r * cols + c, r < rows ? cols - c : 0, fp8_codes(f[i], s, inv, fast));
+  }
+  if (threadIdx.x == 0) scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+}
+
+template <typename T>
+int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int64_t cols,
+                 int block_rows, cudaStream_t s) {
+  const T *in = static_cast<const T *>(x);
+  const bool wide = cols % 8 == 0 && aligned_to(x, 16) && aligned_to(codes, 8);
+  const int64_t row_blocks = (cols + kBlock - 1) / kBlock;
+  if (block_rows == 1) {
+    const int64_t blocks = rows * row_blocks;
+    const int64_t per_cta = kQuantThreads / 16 * 4;
+    const int64_t grid = (blocks + per_cta - 1) / per_cta;
+    if (grid > 0x7fffffffll) return CF_ERR_INVALID_ARGUMENT;
+    if (wide) {
+      fp8_quantize_rows_kernel<T, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
+          in, codes, scales, blocks, cols, row_blocks);
+    } else {
+      fp8_quantize_rows_kernel<T, false><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
+          in, codes, scales, blocks, cols, row_blocks);
+    }
+    return check_launch();
+  }
+  // Bands of at most 65535 row blocks (the grid's limit in y).
+  for (int64_t r = 0; r < rows; r += int64_t{65535} * kBlock) {
+    const int64_t n = std::min<int64_t>(rows - r, int64_t{65535} * kBlock);
+    const dim3 grid(static_cast<unsigned>(row_blocks),
+                    static_cast<unsigned>((n + kBlock - 1) / kBlock));
+    float *to = scales + r / kBlock * row_blocks;
+    if (wide) {
+      fp8_quantize_blocks_kernel<T, true>
+          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n, cols);
+    } else {
+      fp8_quantize_blocks_kernel<T, false>
+          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n, cols);
+    }
+    if (int st = check_launch()) return st;
+  }
+  return CF_OK;
+}
+
+int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, int64_t rows,
+                     int64_t cols, int block_rows, cudaStream_t s) {
+  switch (dtype) {
+    case CF_DTYPE_F32: return quantize_fp8<float>(x, codes, scales, rows, cols, block_rows, s);
+    case CF_DTYPE_BF16:
+      return quantize_fp8<__nv_bfloat16>(x, codes, scales, rows, cols, block_rows, s);
+    default: return quantize_fp8<__half>(x, codes, scales, rows, cols, block_rows, s);
+  }
+}
+
+// ---------------------------------------------------------------- products
+
+struct Fp8Params {
+  const uint8_t *a;      // codes [m, k], or the unquantised x of a fused call
+  const float *a_scales; // [m, kb]
+  const uint8_t *b;      // codes [n, k]
+  const float *b_scales; // [ceil(n / 128), kb]
+  void *y;               // [m, n]
+  int64_t m, n, k;
+  int num_kb;
+  int m_tiles, n_tiles, band;
+  unsigned *err;
+};
+
+// Few rows: bound by reading b once. Each warp takes every kWarps-th 128-block of
+// k of 16 * kMT features and multiplies them with all tokens on the warp-wide
+// MMA (m16n8k32, features as M, tokens as N): at these shapes the tensor core's
+// rate does not matter, and the operands go straight from global memory to
+// registers, next block in flight. A lane's four fragment words of a feature are
+// 16 consecutive bytes: within a block any order of k will do as long as both
+// operands use it. kQuant quantises the tokens on the way (every CTA again,
+// which eight tokens are few enough for), so the call is one launch.
+constexpr int kStreamWarps = 8;
+
+template <typename T, int kNT, int kMT, bool kQuant>
+struct StreamLoads {
+  uint4 w[kMT][2][2];  // [16 features][row g, row g + 8][64-byte half]
+  uint4 x[kNT][kQuant ? 4 : 2];
+};
+
+__device__ __forceinline__ uint4 load_once(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+template <typename T, int kNT, int kMT, bool kQuant>
+__global__ void __launch_bounds__(kStreamWarps *kWarp)
+    fp8_stream_kernel(const Fp8Params p) {
+  constexpr int kFeatures = 16 * kMT;
+  __shared__ float red[kStreamWarps][kNT * 8][kFeatures + 1];
+  const int warp = threadIdx.x / kWarp;
+  const int lane = threadIdx.x % kWarp;
+  const int g = lane / 4, t = lane % 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kFeatures;
+  const float *w_scale = p.b_scales + n0 / kBlock * p.num_kb;
+  const T *x = reinterpret_cast<const T *>(p.a);
+
+  using Loads = StreamLoads<T, kNT, kMT, kQuant>;
+  auto load = [&](Loads &l, int kb) {
+    const int64_t k0 = static_cast<int64_t>(kb) * kBlock + t * 16;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int64_t k = k0 + half * 64;
+      const bool in = k < p.k;  // k is a multiple of 16: all 16 bytes or none
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int64_t n = n0 + mt * 16 + r * 8 + g;
+          l.w[mt][r][half] = in && n < p.n ? load_once(p.b + n * p.k + k) : make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        const int64_t m = nt * 8 + g;
+        const bool ok = in && m < p.m;
+        if constexpr (kQuant) {
+          const uint4 *src = reinterpret_cast<const uint4 *>(x + m * p.k + k);
+          l.x[nt][2 * half] = ok ? __ldg(src) : make_uint4(0, 0, 0, 0);
+          l.x[nt][2 * half + 1] = ok ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+        } else {
+          l.x[nt][half] = ok ? __ldg(reinterpret_cast<const uint4 *>(p.a + m * p.k + k))
+                             : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  float acc[kMT][kNT][4] = {};
+  Loads next;
+  if (warp < p.num_kb) load(next, warp);
+  for (int kb = warp; kb < p.num_kb; kb += kStreamWarps) {
+    const Loads cur = next;
+    if (kb + kStreamWarps < p.num_kb) load(next, kb + kStreamWarps);
+    const float ws = w_scale[kb];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      uint4 xc[2];       // token nt * 8 + g's codes
+      float s0, s1;      // scales of the lane's two result columns, tokens 2t and 2t + 1
+      if constexpr (kQuant) {
+        float f[4][8];
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T *e = reinterpret_cast<const T *>(&cur.x[nt][i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] = as_float<T>(e[j]);
+          m = max(m, absmax_bits(f[i]));
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float s = fp8_scale(m);
+        const float inv = __frcp_rn(s);
+        const bool fast = fp8_fast(m, s);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint2 lo = fp8_codes(f[2 * half], s, inv, fast);
+          const uint2 hi = fp8_codes(f[2 * half + 1], s, inv, fast);
+          xc[half] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+        s0 = __shfl_sync(0xffffffffu, s, 8 * t);
+        s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      } else {
+        xc[0] = cur.x[nt][0];
+        xc[1] = cur.x[nt][1];
+        const int64_t m = nt * 8 + 2 * t;
+        s0 = m < p.m ? __ldg(p.a_scales + m * p.num_kb + kb) : 0.0f;
+        s1 = m + 1 < p.m ? __ldg(p.a_scales + (m + 1) * p.num_kb + kb) : 0.0f;
+      }
+      s0 *= ws;
+      s1 *= ws;
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+        float d[4] = {};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            mma_e4m3(d, word(cur.w[mt][0][half], 2 * j), word(cur.w[mt][1][half], 2 * j),
+                     word(cur.w[mt][0][half], 2 * j + 1), word(cur.w[mt][1][half], 2 * j + 1),
+                     word(xc[half], 2 * j), word(xc[half], 2 * j + 1));
+          }
+        }
+        acc[mt][nt][0] = fmaf(s0, d[0], acc[mt][nt][0]);
+        acc[mt][nt][1] = fmaf(s1, d[1], acc[mt][nt][1]);
+        acc[mt][nt][2] = fmaf(s0, d[2], acc[mt][nt][2]);
+        acc[mt][nt][3] = fmaf(s1, d[3], acc[mt][nt][3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        red[warp][nt * 8 + 2 * t + (i & 1)][mt * 16 + g + (i & 2) * 4] = acc[mt][nt][i];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kNT * 8 * kFeatures; i += kStreamWarps * kWarp) {
+    const int m = i / kFeatures, f = i % kFeatures;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStreamWarps; ++w) v += red[w][m][f];
+    if (m < p.m && n0 + f < p.n) {
+      T *y = static_cast<T *>(p.y) + m * p.n + n0 + f;
+      if constexpr (std::is_same_v<T, __half>) {
+        *y = __float2half_rn(v);
+      } else {
+        *y = __float2bfloat16_rn(v);
+      }
+    }
+  }
+}
+
+constexpr int64_t kFusedRows = 8;    // quantised inside the streaming kernel
+constexpr int64_t kStreamRows = 32;  // streamed at all; tiles above
+
+template <typename T, int kNT, bool kQuant>
+int launch_stream(const Fp8Params &p, cudaStream_t s) {
+  // 32 features a CTA halve the work on the tokens; 16 where that leaves SMs idle.
+  // (Four token tiles leave registers for 16 alone.)
+  const int64_t two = (p.n + 31) / 32;
+  if (kNT <= 2 && two >= sm_count()) {
+    fp8_stream_kernel<T, kNT <= 2 ? kNT : 1, 2, kQuant>
+        <<<static_cast<unsigned>(two), kStreamWarps * kWarp, 0, s>>>(p);
+  } else {
+    fp8_stream_kernel<T, kNT, 1, kQuant>
+        <<<static_cast<unsigned>((p.n + 15) / 16), kStreamWarps * kWarp, 0, s>>>(p);
+  }
+  return check_launch();
+}
+
+// Many rows: 128-token x 256-feature tiles on tcgen05. One MMA group of four
+// (K = 32 each) covers a 128-block of k into one of two TMEM buffers; eight
+// epilogue warps (a thread is a token and half the tile's features) read each
+// finished block, multiply by a_scale b_scale and add into registers while the
+// next block is computed into the other buffer. Half a tile's features are one
+// 128-row block of b, so a thread's scale of a block is one number.
+constexpr int kTileM = 128, kTileN = 256;
+constexpr int kTileThreads = 384;  // warps 0-7 epilogue, 8 producer, 9 MMA, 10-11 idle
+// Registers of an epilogue and of another thread: a share of the 168 that 384
+// threads start with (2 * 216 + 72 = 3 * 168), since an epilogue thread holds
+// 128 fp32 sums.
+constexpr int kTileEpilogueRegs = 216, kTileOtherRegs = 72;
+constexpr int kTileStages = 4;
+constexpr int kTileABytes = kTileM * kBlock;
+constexpr int kTileStageBytes = (kTileM + kTileN) * kBlock;
+constexpr size_t kTileSmem = 1024 + static_cast<size_t>(kTileStages) * kTileStageBytes + 256;
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
+                    const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kTileStages * kTileStageBytes);
+  uint64_t *empty = full + kTileStages;
+  uint64_t *tmem_full = empty + kTileStages;  // [2]
+  uint64_t *tmem_empty = tmem_full + 2;       // [2]
+  uint64_t *drain = tmem_empty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
+  const int warp = threadIdx.x / kWarp;
+  const int lane = threadIdx.x % kWarp;
+  const int tiles = p.m_tiles * p.n_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kTileStages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&tmem_full[i], 1);
+      ptx::mbar_init(&tmem_empty[i], 8);
+    }
+    ptx::mbar_init(drain, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 8 && lane == 0) {
+    ptx::prefetch_tensor_map(&tm_a);
+    ptx::prefetch_tensor_map(&tm_b);
+  }
+  if (warp == 9) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) ptx::lower_registers<kTileOtherRegs>();
+  if (warp == 8) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, outstanding = 0, parities = 0;
+      for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+        int tm, tn;
+        band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
+            record_timeout(p.err, abort_flag);
+            break;
+          }
+          uint8_t *sa = smem + stage * kTileStageBytes;
+          ptx::mbar_expect_tx(&full[stage], kTileStageBytes);
+          ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, tm * kTileM);
+          ptx::tma_load_2d(sa + kTileABytes, &tm_b, &full[stage], kb * kBlock, tn * kTileN);
+          outstanding |= 1u << stage;
+          parities = (parities & ~(1u << stage)) | (phase << stage);
+          if (++stage == kTileStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (aborted(abort_flag)) {
+        for (int s = 0; s < kTileStages; ++s) {
+          if (outstanding & (1u << s)) {
+            ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
+          }
+        }
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::make_idesc_e4m3(kTileM, kTileN);
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!ptx::mbar_wait(&tmem_empty[buf], buf_phase ^ 1) ||
+              !ptx::mbar_wait(&full[stage], phase)) {
+            record_timeout(p.err, abort_flag);
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_addr(smem + stage * kTileStageBytes);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            ptx::mma_f8f6f4(tmem + buf * kTileN, kmajor_desc(sa, 128, ks),
+                            kmajor_desc(sa + kTileABytes, 128, ks), idesc, ks > 0);
+          }
+          ptx::mma_commit(&empty[stage]);
+          ptx::mma_commit(&tmem_full[buf]);
+          if (++stage == kTileStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (++buf == 2) {
+            buf = 0;
+            buf_phase ^= 1;
+          }
+        }
+      }
+      if (aborted(abort_flag)) {
+        ptx::mma_commit(drain);
+        ptx::mbar_wait(drain, 0, 200000000ull);
+      }
+    }
+  } else if (warp < 8) {
+    ptx::raise_registers<kTileEpilogueRegs>();
+    const int quarter = warp % 4, half = warp / 4;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+      int tm, tn;
+      band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
+      const int64_t row = static_cast<int64_t>(tm) * kTileM + quarter * 32 + lane;
+      const int64_t col0 = static_cast<int64_t>(tn) * kTileN + half * 128;
+      const float *a_scale = p.a_scales + (row < p.m ? row : 0) * p.num_kb;
+      const float *b_scale = p.b_scales + (col0 < p.n ? col0 / kBlock : 0) * p.num_kb;
+      uint64_t acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = 0;
+      float scale = a_scale[0] * b_scale[0];
+      bool ok = true;
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        const int ahead = kb + 1 < p.num_kb ? kb + 1 : kb;
+        const float next = __ldg(a_scale + ahead) * __ldg(b_scale + ahead);
+        ok = ptx::warp_wait(&tmem_full[buf], buf_phase);
+        if (!ok) {
+          if (lane == 0) record_timeout(p.err, abort_flag);
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint64_t s2 = ptx::splat_f32x2(scale);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32b_x32(t_row + buf * kTileN + c * 32, v);
+          ptx::tmem_ld_wait();
+          if (c == 3) {
+            ptx::tc_fence_before();
+            ptx::warp_arrive(&tmem_empty[buf]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t d = ptx::pack_f32x2(__uint_as_float(v[2 * e]),
+                                               __uint_as_float(v[2 * e + 1]));
+            acc[c * 16 + e] = ptx::fma_f32x2(s2, d, acc[c * 16 + e]);
+          }
+        }
+        scale = next;
+        if (++buf == 2) {
+          buf = 0;
+          buf_phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (row < p.m) {
+        uint16_t *out = static_cast<uint16_t *>(p.y) + row * p.n + col0;
+        const bool wide = p.n % 8 == 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = ptx::unpack_f32x2(acc[c * 4 + e]);
+            w[e] = kBf16 ? ptx::pack_bf16x2(f.x, f.y) : ptx::pack_f16x2(f.x, f.y);
+          }
+          if (wide) {
+            if (col0 + c * 8 < p.n) {
+              *reinterpret_cast<uint4 *>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (col0 + c * 8 + e < p.n) {
+                out[c * 8 + e] = static_cast<uint16_t>(w[e / 2] >> (e % 2 * 16));
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool kBf16>
+int launch_tiles(Fp8Params p, cudaStream_t s) {
+  p.m_tiles = static_cast<int>((p.m + kTileM - 1) / kTileM);
+  p.n_tiles = static_cast<int>((p.n + kTileN - 1) / kTileN);
+  // As many row blocks of a in a band as stay in L2 while b streams past.
+  const int64_t fit = (int64_t{32} << 20) / (kTileM * std::max<int64_t>(p.k, 1));
+  p.band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, fit)));
+  p.err = device_error_word();
+  if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
+  CUtensorMap tm_a, tm_b;
+  if (int st = make_map(&tm_a, p.a, 1, p.k, p.m, kBlock, kTileM, true)) return st;
+  if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, kTileN, true)) return st;
+  if (int st = allow_dynamic_smem<fp8_tile_kernel<kBf16>>(kTileSmem)) return st;
+  const unsigned grid = static_cast<unsigned>(
+      std::min<int64_t>(static_cast<int64_t>(p.m_tiles) * p.n_tiles, sm_count()));
+  fp8_tile_kernel<kBf16><<<grid, kTileThreads, kTileSmem, s>>>(tm_a, tm_b, p);
+  return check_launch();
+}
+
+template <typename T>
+int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
+  if (p.m <= 8) return launch_stream<T, 1, false>(p, s);
+  if (p.m <= 16) return launch_stream<T, 2, false>(p, s);
+  if (p.m <= kStreamRows) return launch_stream<T, 4, false>(p, s);
+  return launch_tiles<std::is_same_v<T, __nv_bfloat16>>(p, s);
+}
+
+int check_fp8_shape(int64_t m, int64_t k, int64_t n, int dtype) {
+  if (m < 0 || k < 0 || n < 0) return CF_ERR_INVALID_ARGUMENT;
+  if (dtype != CF_DTYPE_BF16 && dtype != CF_DTYPE_F16) return CF_ERR_UNSUPPORTED;
+  if (m == 0 || n == 0) return CF_OK;
+  if (k == 0 || k % 16 != 0) return CF_ERR_UNSUPPORTED;
+  if (m > 0x7fffffffll - kTileM || n > 0x7fffffffll - kTileN || k > 0x7fffffffll - kBlock ||
+      (m + kTileM - 1) / kTileM * ((n + kTileN - 1) / kTileN) > 0x7fffffffll) {
+    return CF_ERR_INVALID_ARGUMENT;  // tile counts and coordinates are 32-bit
+  }
+  return CF_OK;
+}
+
+Fp8Params fp8_params(const void *a, const float *a_scales, const uint8_t *b, const float *b_scales,
+                     void *y, int64_t m, int64_t k, int64_t n) {
+  Fp8Params p{};
+  p.a = static_cast<const uint8_t *>(a);
+  p.a_scales = a_scales;
+  p.b = b;
+  p.b_scales = b_scales;
+  p.y = y;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.num_kb = static_cast<int>((k + kBlock - 1) / kBlock);
+  return p;
+}
+
+size_t fp8_code_bytes(int64_t m, int64_t k) {
+  return (static_cast<size_t>(m) * static_cast<size_t>(k) + 255) & ~static_cast<size_t>(255);
+}
+
+}  // namespace
+}  // namespace cfb
+
+extern "C" {
+
+int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales, int64_t rows,
+                    int64_t cols, int block_rows, cf_stream_t stream) {
+  if (rows < 0 || cols < 0) return CF_ERR_INVALID_ARGUMENT;
+  if (dtype != CF_DTYPE_F32 && dtype != CF_DTYPE_BF16 && dtype != CF_DTYPE_F16) {
+    return CF_ERR_UNSUPPORTED;
+  }
+  if (block_rows != 1 && block_rows != CF_FP8_BLOCK_SIZE) return CF_ERR_UNSUPPORTED;
+  if (rows == 0 || cols == 0) return CF_OK;
+  if (!input || !codes || !scales) return CF_ERR_INVALID_ARGUMENT;
+  if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 37)) {
+    return CF_ERR_INVALID_ARGUMENT;
+  }
+  return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows,
+                               reinterpret_cast<cudaStream_t>(stream));
+}
+
+int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, const uint8_t *b_codes,
+                  const float *b_scales, void *y, int64_t m, int64_t k, int64_t n, int dtype,
+                  cf_stream_t stream) {
+  if (int st = cfb::check_fp8_shape(m, k, n, dtype)) return st;
+  if (m == 0 || n == 0) return CF_OK;
+  if (!a_codes || !a_scales || !b_codes || !b_scales || !y) return CF_ERR_INVALID_ARGUMENT;
+  if (!cfb::aligned_to(a_codes, 16) || !cfb::aligned_to(b_codes, 16) || !cfb::aligned_to(y, 16)) {
+    return CF_ERR_MISALIGNED;
+  }
+  const cfb::Fp8Params p = cfb::fp8_params(a_codes, a_scales, b_codes, b_scales, y, m, k, n);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == CF_DTYPE_BF16 ? cfb::matmul_fp8<__nv_bfloat16>(p, s)
+                                : cfb::matmul_fp8<__half>(p, s);
+}
+
+size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k) {
+  if (m <= cfb::kFusedRows || k <= 0) return 0;
+  const int64_t blocks = m * ((k + cfb::kBlock - 1) / cfb::kBlock);
+  return cfb::fp8_code_bytes(m, k) + static_cast<size_t>(blocks) * sizeof(float);
+}
+
+int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, void *y, int64_t m,
+                  int64_t k, int64_t n, int dtype, void *workspace, size_t workspace_bytes,
+                  cf_stream_t stream) {
+  if (int st = cfb::check_fp8_shape(m, k, n, dtype)) return st;
+  if (m == 0 || n == 0) return CF_OK;
+  if (!x || !w_codes || !w_scales || !y) return CF_ERR_INVALID_ARGUMENT;
+  if (!cfb::aligned_to(x, 16) || !cfb::aligned_to(w_codes, 16) || !cfb::aligned_to(y, 16)) {
+    return CF_ERR_MISALIGNED;
+  }
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (m <= cfb::kFusedRows) {
+    const cfb::Fp8Params p = cfb::fp8_params(x, nullptr, w_codes, w_scales, y, m, k, n);
+    return dtype == CF_DTYPE_BF16 ? cfb::launch_stream<__nv_bfloat16, 1, true>(p, s)
+                                  : cfb::launch_stream<__half, 1, true>(p, s);
+  }
+  if (workspace == nullptr || workspace_bytes < cf_linear_fp8_workspace_bytes(m, k)) {
+    return CF_ERR_WORKSPACE;
+  }
+  if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
+  uint8_t *codes = static_cast<uint8_t *>(workspace);
+  float *scales = reinterpret_cast<float *>(codes + cfb::fp8_code_bytes(m, k));
+  if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, s)) return st;
+  return cf_matmul_fp8(codes, scales, w_codes, w_scales, y, m, k, n, dtype, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,121 @@
+// Pieces shared by the tensor-core kernels: operand descriptors, the abort
+// protocol of their bounded waits, tile order, tensor maps and launch attributes.
+#pragma once
+
+#include <cuda.h>
+
+#include <atomic>
+
+#include "cf_common.cuh"
+#include "ptx.cuh"
+
+namespace cfb {
+namespace {
+
+__device__ __forceinline__ uint32_t swizzle_for_row_bytes(int row_bytes) {
+  return row_bytes >= 128 ? ptx::kSwizzle128B : row_bytes == 64 ? ptx::kSwizzle64B
+                                                                 : ptx::kSwizzle32B;
+}
+
+// Shared-memory descriptor of a K-major operand whose rows are `row_bytes`
+// (32/64/128) long and swizzled at that width; 8-row core groups are
+// 8 * row_bytes apart. k-step `ks` (16 elements = 32 bytes) advances the start
+// address inside the swizzle atom.
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t base, int row_bytes, int ks) {
+  return ptx::make_smem_desc(base + ks * 32, 16, 8 * row_bytes, swizzle_for_row_bytes(row_bytes));
+}
+
+// Descriptor of an MN-major operand stored as chunks of `chunk_elems` MN
+// elements (chunk_elems * 2 = row bytes, swizzled at that width) x k rows;
+// chunks are `chunk_stride` bytes apart. k-step `ks` = 16 rows further.
+__device__ __forceinline__ uint64_t mnmajor_desc(uint32_t base, int row_bytes, int chunk_stride,
+                                                 int ks) {
+  return ptx::make_smem_desc(base + ks * 16 * row_bytes, chunk_stride, 8 * row_bytes,
+                             swizzle_for_row_bytes(row_bytes));
+}
+
+__device__ __forceinline__ void record_timeout(unsigned *err, int *abort_flag) {
+  atomicOr(err, kDevErrTimeout);
+  *reinterpret_cast<volatile int *>(abort_flag) = 1;
+}
+
+__device__ __forceinline__ bool aborted(const int *abort_flag) {
+  return *reinterpret_cast<const volatile int *>(abort_flag) != 0;
+}
+
+// Tile t of a grid of `rows` x `cols` tiles, walked in bands of `band` rows
+// with the row index fastest inside a band: the CTAs of one wave then share
+// a few column blocks (each read from DRAM about once per band) while the
+// band's row blocks stay resident in L2.
+__device__ __forceinline__ void band_order(int t, int rows, int cols, int band, int &row,
+                                           int &col) {
+  const int per_band = band * cols;
+  const int b = t / per_band;
+  const int in_band = min(band, rows - b * band);
+  const int i = t - b * per_band;
+  row = b * band + i % in_band;
+  col = i / in_band;
+}
+
+// ---- host: tensor maps and launches
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                   const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static std::atomic<EncodeTiledFn> cached{nullptr};
+  EncodeTiledFn fn = cached.load(std::memory_order_acquire);
+  if (fn != nullptr) return fn;
+  void *sym = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) !=
+          cudaSuccess ||
+      q != cudaDriverEntryPointSuccess || sym == nullptr) {
+    return nullptr;
+  }
+  fn = reinterpret_cast<EncodeTiledFn>(sym);
+  cached.store(fn, std::memory_order_release);
+  return fn;
+}
+
+// Launch attribute of the linear kernels: they may begin while the
+// down-projection launched just before them on the stream is still running
+// (their producers wait for it before reading P).
+inline void set_programmatic_dependency(cudaLaunchAttribute &attr) {
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+}
+
+inline CUtensorMapSwizzle swizzle_for(int inner_bytes) {
+  switch (inner_bytes) {
+    case 32: return CU_TENSOR_MAP_SWIZZLE_32B;
+    case 64: return CU_TENSOR_MAP_SWIZZLE_64B;
+    case 128: return CU_TENSOR_MAP_SWIZZLE_128B;
+    default: return CU_TENSOR_MAP_SWIZZLE_NONE;
+  }
+}
+
+// 2-D row-major tensor [outer, inner] with element size esize and rows `ld` elements apart
+// (0: inner), box [box_outer, box_inner].
+inline int make_map(CUtensorMap *map, const void *base, int esize, int64_t inner, int64_t outer,
+                    int box_inner, int box_outer, bool swizzle, int64_t ld = 0) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return record_cuda_error(cudaErrorNotSupported);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld ? ld : inner) * esize};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType dt = esize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  const CUresult r = fn(map, dt, 2, const_cast<void *>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle ? swizzle_for(box_inner * esize) : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CF_OK : CF_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace cfb

@@ -255,6 +255,18 @@ __device__ __forceinline__ void mma_tf32(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
+// D (TMEM, fp32) [+]= A * B with 8-bit operands whose formats the instruction
+// descriptor names (kind::f8f6f4, K = 32).
+__device__ __forceinline__ void mma_f8f6f4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // fp32 rounded to the nearest tf32 (10 explicit mantissa bits, ties away).
 __device__ __forceinline__ float round_tf32(float v) {
   uint32_t r;
@@ -297,6 +309,18 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Moves registers between the warpgroups of a CTA (every warp of a warpgroup
+// executes it). The shares may not add up to more than the CTA started with.
+template <int kRegs>
+__device__ __forceinline__ void raise_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+template <int kRegs>
+__device__ __forceinline__ void lower_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // Named barrier `id` over `count` threads (a multiple of 32).
@@ -390,6 +414,13 @@ __host__ __device__ constexpr uint32_t make_idesc_tf32(int m, int n, bool a_mn_m
                                                        bool b_mn_major) {
   return (1u << 4) | (2u << 7) | (2u << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | ((static_cast<uint32_t>(n) >> 3) << 17) |
+         ((static_cast<uint32_t>(m) >> 4) << 24);
+}
+
+// Instruction descriptor of kind::f8f6f4 with fp32 accumulation, K-major e4m3
+// operands (A and B format code 0; other fields as make_idesc_f16).
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
+  return (1u << 4) | ((static_cast<uint32_t>(n) >> 3) << 17) |
          ((static_cast<uint32_t>(m) >> 4) << 24);
 }
 

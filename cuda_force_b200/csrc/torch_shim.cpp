@@ -527,6 +527,123 @@ std::vector<at::Tensor> gated_residual_rmsnorm_autograd(
                                      residual_scale, eps);
 }
 
+// ---- 8-bit floating point
+
+std::vector<at::Tensor> quantize_fp8_cuda(const at::Tensor &input, int64_t block_rows) {
+  check_cuda(input, "input");
+  check_contiguous(input, "input");
+  const int dtype = dtype_code(input, "input");
+  TORCH_CHECK(block_rows == 1 || block_rows == CF_FP8_BLOCK_SIZE, "block_rows must be 1 or ",
+              CF_FP8_BLOCK_SIZE, ", got ", block_rows);
+  TORCH_CHECK(input.dim() >= 1 && (block_rows == 1 || input.dim() == 2),
+              "input must be 2-D for square blocks, got ", input.dim(), " dimensions");
+  const c10::cuda::CUDAGuard guard(input.device());
+  const int64_t cols = input.size(-1), rows = cols > 0 ? input.numel() / cols : 0;
+  std::vector<int64_t> scale_shape(input.sizes().begin(), input.sizes().end());
+  scale_shape.back() = (cols + CF_FP8_BLOCK_SIZE - 1) / CF_FP8_BLOCK_SIZE;
+  if (block_rows > 1) scale_shape[0] = (scale_shape[0] + block_rows - 1) / block_rows;
+  at::Tensor codes = at::empty(input.sizes(), input.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scales = at::empty(scale_shape, input.options().dtype(at::kFloat));
+  check_status(cf_quantize_fp8(input.const_data_ptr(), dtype,
+                               static_cast<uint8_t *>(codes.data_ptr()), scales.data_ptr<float>(),
+                               rows, cols, static_cast<int>(block_rows), current_stream()),
+               "quantize_fp8");
+  return {codes, scales};
+}
+
+// Codes [rows, k] with k zero-padded to a multiple of 16 bytes, the unit of the
+// kernels' row strides; zeros leave the product unchanged and k stays in the
+// same number of 128-blocks.
+at::Tensor padded_codes(const at::Tensor &t, int64_t kp) {
+  if (t.size(1) == kp) return t;
+  at::Tensor out = at::zeros({t.size(0), kp}, t.options());
+  out.narrow(1, 0, t.size(1)).copy_(t);
+  return out;
+}
+
+void check_fp8_operand(const at::Tensor &codes, const at::Tensor &scales, const char *name,
+                       int64_t block_rows) {
+  check_cuda(codes, name);
+  check_cuda(scales, name);
+  TORCH_CHECK(codes.dim() == 2, name, " codes must be 2-D, got ", codes.dim(), " dimensions");
+  TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn, name, " codes must be float8_e4m3fn, got ",
+              codes.scalar_type());
+  TORCH_CHECK(scales.scalar_type() == at::kFloat, name, " scales must be float32, got ",
+              scales.scalar_type());
+  check_contiguous(codes, name);
+  check_contiguous(scales, name);
+  TORCH_CHECK(codes.device() == scales.device(), name, " codes and scales must share a device");
+  const int64_t want = (codes.size(0) + block_rows - 1) / block_rows *
+                       ((codes.size(1) + CF_FP8_BLOCK_SIZE - 1) / CF_FP8_BLOCK_SIZE);
+  TORCH_CHECK(scales.numel() == want, "expected ", want, " block scales of ", name, ", got ",
+              scales.numel());
+}
+
+const uint8_t *code_ptr(const at::Tensor &t) {
+  return static_cast<const uint8_t *>(t.const_data_ptr());
+}
+
+// A copy where the kernels' 16-byte alignment is not met (a slice of a larger tensor).
+at::Tensor aligned16(const at::Tensor &t) {
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
+at::Tensor matmul_fp8_cuda(const at::Tensor &a_codes, const at::Tensor &a_scales,
+                           const at::Tensor &b_codes, const at::Tensor &b_scales,
+                           at::ScalarType dtype) {
+  check_fp8_operand(a_codes, a_scales, "a", 1);
+  check_fp8_operand(b_codes, b_scales, "b", CF_FP8_BLOCK_SIZE);
+  TORCH_CHECK(a_codes.device() == b_codes.device(), "a and b must share a device");
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf,
+              "dtype must be bfloat16 or float16, got ", dtype);
+  const int64_t m = a_codes.size(0), k = a_codes.size(1), n = b_codes.size(0);
+  TORCH_CHECK(b_codes.size(1) == k, "b codes must be [n, ", k, "], got ", b_codes.sizes());
+  const c10::cuda::CUDAGuard guard(a_codes.device());
+  at::Tensor y = at::empty({m, n}, a_codes.options().dtype(dtype));
+  if (k == 0) return y.zero_();
+  const int64_t kp = (k + 15) / 16 * 16;
+  const at::Tensor a = aligned16(padded_codes(a_codes, kp));
+  const at::Tensor b = aligned16(padded_codes(b_codes, kp));
+  check_status(cf_matmul_fp8(code_ptr(a), a_scales.data_ptr<float>(), code_ptr(b),
+                             b_scales.data_ptr<float>(), y.data_ptr(), m, kp, n,
+                             dtype == at::kBFloat16 ? CF_DTYPE_BF16 : CF_DTYPE_F16,
+                             current_stream()),
+               "matmul_fp8");
+  return y;
+}
+
+// x [m, k] float16 or bfloat16, quantised on the way; w codes [n, k].
+at::Tensor linear_fp8_cuda(const at::Tensor &x, const at::Tensor &w_codes,
+                           const at::Tensor &w_scales) {
+  check_cuda(x, "x");
+  check_contiguous(x, "x");
+  check_fp8_operand(w_codes, w_scales, "w", CF_FP8_BLOCK_SIZE);
+  TORCH_CHECK(x.dim() == 2, "x must be 2-D, got ", x.dim(), " dimensions");
+  const int dtype = dtype_code(x, "x");
+  TORCH_CHECK(dtype != CF_DTYPE_F32, "linear_fp8: x must be bfloat16 or float16");
+  TORCH_CHECK(x.device() == w_codes.device(), "x and w must share a device");
+  const int64_t m = x.size(0), k = x.size(1), n = w_codes.size(0);
+  TORCH_CHECK(w_codes.size(1) == k, "w codes must be [n, ", k, "], got ", w_codes.sizes());
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = at::empty({m, n}, x.options());
+  if (k == 0) return y.zero_();
+  const int64_t kp = (k + 15) / 16 * 16;
+  at::Tensor xp = x;
+  if (kp != k) {
+    xp = at::zeros({m, kp}, x.options());
+    xp.narrow(1, 0, k).copy_(x);
+  }
+  xp = aligned16(xp);
+  const at::Tensor w = aligned16(padded_codes(w_codes, kp));
+  const size_t ws_bytes = cf_linear_fp8_workspace_bytes(m, kp);
+  at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+  check_status(cf_linear_fp8(xp.const_data_ptr(), code_ptr(w), w_scales.data_ptr<float>(),
+                             y.data_ptr(), m, kp, n, dtype, ws.data_ptr(), ws_bytes,
+                             current_stream()),
+               "linear_fp8");
+  return y;
+}
+
 // ---- host tensors: the reference semantics (python/cudaforge/ops.py:164-240)
 
 std::vector<at::Tensor> quantize_int8_host(const at::Tensor &input) {
@@ -630,13 +747,18 @@ TORCH_LIBRARY(cudaforge, m) {
   m.def(
       "gated_residual_rmsnorm(Tensor x, Tensor residual, Tensor weight, Tensor? post_weight, "
       "Tensor? gate, int gate_groups, float residual_scale, float eps) -> Tensor[]");
+  m.def("quantize_fp8(Tensor input, int block_rows) -> Tensor[]");
+  m.def(
+      "matmul_fp8(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, "
+      "ScalarType dtype) -> Tensor");
+  m.def("linear_fp8(Tensor x, Tensor w_codes, Tensor w_scales) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
   for (const char *name : {"lora_linear", "quantize_int8", "dequantize_int8", "lora_linear_int8",
                            "quantize_dequantize", "quantize_int8_many", "rmsnorm",
                            "fused_residual_rmsnorm", "softmax", "sum", "silu", "gelu",
-                           "swiglu"}) {
+                           "swiglu", "quantize_fp8", "matmul_fp8", "linear_fp8"}) {
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
   }
   m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_autograd);
@@ -652,6 +774,9 @@ TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
   m.impl("rmsnorm", &rmsnorm_cuda);
   m.impl("fused_residual_rmsnorm", &fused_residual_rmsnorm_cuda);
   m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_cuda);
+  m.impl("quantize_fp8", &quantize_fp8_cuda);
+  m.impl("matmul_fp8", &matmul_fp8_cuda);
+  m.impl("linear_fp8", &linear_fp8_cuda);
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CompositeExplicitAutograd, m) {

@@ -23,9 +23,10 @@ three differences that are deliberate:
 the reference's names, arguments and messages and take all three dtypes.
 
 Additive ops: ``lora_linear_int8`` (W as block-INT8 codes + scales),
-``quantize_dequantize`` (fake quantisation), ``quantize_int8_many`` and, around a
+``quantize_dequantize`` (fake quantisation), ``quantize_int8_many`` and, for a
 transformer's feed-forward block, ``gated_residual_rmsnorm``, which is
-differentiable.
+differentiable, and the 8-bit floating-point ``quantize_fp8``, ``matmul_fp8``
+and ``linear_fp8``.
 """
 
 from __future__ import annotations
@@ -40,6 +41,10 @@ import torch
 # cuda_force_b200/csrc/cf_common.cuh and CF_QUANT_BLOCK_SIZE in
 # include/cudaforge_b200.h.
 QUANT_BLOCK_SIZE = 64
+
+# Block size of the 8-bit floating-point formats. Must match CF_FP8_BLOCK_SIZE in
+# include/cudaforge_b200.h.
+FP8_BLOCK_SIZE = 128
 
 _SHIM = Path(__file__).resolve().parent / "_C.so"
 
@@ -572,3 +577,92 @@ def lora_linear_int8(
         _as_stored(lora_b), float(scale)
     )
     return y.reshape(*lead, y.shape[-1])
+
+
+def _fp8_scale_shape(shape: tuple[int, ...], block_rows: int) -> tuple[int, ...]:
+    return (*shape[:-2], -(-shape[-2] // block_rows), -(-shape[-1] // FP8_BLOCK_SIZE))
+
+
+def _check_fp8_operand(name: str, codes: torch.Tensor, scales: torch.Tensor,
+                       block_rows: int) -> None:
+    if codes.ndim != 2 or codes.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{name}_codes must be a 2-D float8_e4m3fn tensor, got {codes.dtype} "
+                         f"{tuple(codes.shape)}")
+    expected = _fp8_scale_shape(tuple(codes.shape), block_rows)
+    if tuple(scales.shape) != expected or scales.dtype != torch.float32:
+        raise ValueError(f"expected float32 block scales {expected} for {name}_codes "
+                         f"{tuple(codes.shape)}, got {scales.dtype} {tuple(scales.shape)}")
+
+
+def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    """8-bit floating-point quantisation with a float32 scale for each block.
+
+    Blocks are ``block_rows x FP8_BLOCK_SIZE``: 1 row for activations ``[...,
+    features]``, ``FP8_BLOCK_SIZE`` rows for a weight ``[out_features,
+    in_features]``. ``scale = absmax / 448`` (1 for a block of zeros) and ``code =
+    e4m3(x / scale)``, nearest even, saturating. Returns ``(codes, scales)``:
+    ``float8_e4m3fn`` shaped like ``x``, and ``[..., ceil(features / 128)]`` or
+    ``[ceil(out / 128), ceil(in / 128)]``. The last block of a row or column may
+    be smaller.
+    """
+    if block_rows not in (1, FP8_BLOCK_SIZE):
+        raise ValueError(f"block_rows must be 1 or {FP8_BLOCK_SIZE}, got {block_rows}")
+    if x.ndim < 1 or (block_rows > 1 and x.ndim != 2):
+        raise ValueError(f"x must be [..., features], or 2-D for square blocks, got "
+                         f"{tuple(x.shape)}")
+    if x.dtype not in KERNEL_DTYPES:
+        raise ValueError(f"quantize_fp8 takes float32, float16 or bfloat16 tensors, got {x.dtype}")
+    _require("quantize_fp8", x)
+    codes, scales = torch.ops.cudaforge.quantize_fp8(x.contiguous(), block_rows)
+    return codes, scales
+
+
+def matmul_fp8(
+    a_codes: torch.Tensor,
+    a_scales: torch.Tensor,
+    b_codes: torch.Tensor,
+    b_scales: torch.Tensor,
+    dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``a @ b.T`` of operands that :func:`quantize_fp8` made.
+
+    Args:
+        a_codes, a_scales: ``[m, k]`` in blocks of 1 row.
+        b_codes, b_scales: ``[n, k]`` (nn.Linear layout) in blocks of 128 rows.
+        dtype: bfloat16 or float16, the type of the result ``[m, n]``.
+
+    Products of codes are summed over each block of k and scaled in fp32. ``k``
+    that is not a multiple of 16 costs a zero-padded copy of both operands.
+    """
+    _check_fp8_operand("a", a_codes, a_scales, 1)
+    _check_fp8_operand("b", b_codes, b_scales, FP8_BLOCK_SIZE)
+    if a_codes.shape[1] != b_codes.shape[1]:
+        raise ValueError(f"a_codes has {a_codes.shape[1]} input features but b_codes expects "
+                         f"{b_codes.shape[1]}")
+    if dtype not in INT8_LINEAR_DTYPES:
+        raise ValueError(f"matmul_fp8 returns float16 or bfloat16, not {dtype}")
+    _require("matmul_fp8", a_codes, a_scales, b_codes, b_scales)
+    return torch.ops.cudaforge.matmul_fp8(a_codes.contiguous(), a_scales.contiguous(),
+                                          b_codes.contiguous(), b_scales.contiguous(), dtype)
+
+
+def linear_fp8(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """``matmul_fp8(*quantize_fp8(x), w_codes, w_scales, x.dtype)`` for ``x [..., in_features]``.
+
+    ``w_codes [out_features, in_features]`` and ``w_scales`` are
+    ``quantize_fp8(weight, block_rows=128)``; ``x`` is float16 or bfloat16 and is
+    quantised in blocks of 1 x 128 on the way (in the same launch for up to eight
+    rows).
+    """
+    _check_fp8_operand("w", w_codes, w_scales, FP8_BLOCK_SIZE)
+    if x.ndim < 1 or x.shape[-1] != w_codes.shape[1]:
+        raise ValueError(f"x has {x.shape[-1] if x.ndim else 0} input features but weight "
+                         f"expects {w_codes.shape[1]}")
+    if x.dtype not in INT8_LINEAR_DTYPES:
+        raise ValueError("linear_fp8 takes float16 or bfloat16 activations")
+    _require("linear_fp8", x, w_codes, w_scales)
+    lead = x.shape[:-1]
+    y = torch.ops.cudaforge.linear_fp8(
+        x.reshape(math.prod(lead), x.shape[-1]).contiguous(), w_codes.contiguous(),
+        w_scales.contiguous())
+    return y.view(*lead, y.shape[-1])

@@ -329,6 +329,41 @@ CF_API int cf_gated_residual_rmsnorm_backward(
     void *d_post_weight, void *d_gate, int64_t rows, int64_t cols, float residual_scale, int dtype,
     void *workspace, size_t workspace_bytes, cf_stream_t stream);
 
+/* ---- 8-bit floating point ------------------------------------------------ */
+
+/* Elements of a row that share a scale, and rows of a weight that do. */
+#define CF_FP8_BLOCK_SIZE 128
+
+/* Quantises input [rows, cols] (f32, f16 or bf16, contiguous) to e4m3 codes in
+ * blocks of block_rows (1 or CF_FP8_BLOCK_SIZE) x CF_FP8_BLOCK_SIZE elements:
+ *   scale = fl32(absmax / 448), replaced by 1 when it is not > 0
+ *   code  = e4m3(fl32(x / scale)), nearest even, saturating, NaN kept
+ * Blocks at the end of a row or column may be smaller. codes: one byte each,
+ * [rows, cols]; scales: float [ceil(rows / block_rows)][ceil(cols / 128)]. Any
+ * alignment works; a 16-byte aligned input, 8-byte aligned codes and cols % 8 ==
+ * 0 take the vector path. No counterpart in the reference. */
+CF_API int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
+                           int64_t rows, int64_t cols, int block_rows, cf_stream_t stream);
+
+/* y[m, n] = sum_k a[m, k] b[n, k] with a in blocks of 1 x 128 (a_scales float
+ * [m][ceil(k / 128)]) and b in blocks of 128 x 128 (b_scales float
+ * [ceil(n / 128)][ceil(k / 128)]), as cf_quantize_fp8 makes them; products of
+ * codes are summed over each block in fp32 and scaled in fp32; y is of dtype
+ * (f16 or bf16). Requirements: k a positive multiple of 16, codes and y 16-byte
+ * aligned. No counterpart in the reference. */
+CF_API int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, const uint8_t *b_codes,
+                         const float *b_scales, void *y, int64_t m, int64_t k, int64_t n,
+                         int dtype, cf_stream_t stream);
+
+/* cf_quantize_fp8 of x [m, k] (dtype f16 or bf16) in blocks of 1 x 128, then
+ * cf_matmul_fp8 with the weight w [n, k] (nn.Linear layout). Up to 8 rows are
+ * one launch and need no workspace; otherwise the codes and scales of x go to
+ * `workspace` (cf_linear_fp8_workspace_bytes, 16-byte aligned). x 16-byte aligned. */
+CF_API size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k);
+CF_API int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, void *y,
+                         int64_t m, int64_t k, int64_t n, int dtype, void *workspace,
+                         size_t workspace_bytes, cf_stream_t stream);
+
 /* Allocation-free form of cf_lora_linear, for callers that cannot allocate the
  * workspace: hosts whose device memory is reserved up front by another
  * allocator, foreign-language hosts without a CUDA allocator, and loops that

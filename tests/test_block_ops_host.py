@@ -70,3 +70,68 @@ def test_gated_residual_rmsnorm_entry_points_refuse():
     assert bwd(ws_bytes=16) == _abi.CF_ERR_WORKSPACE
     assert bwd(ws=ctypes.c_void_p(0x1008)) == _abi.CF_ERR_MISALIGNED
     assert bwd(rows=0) == _abi.CF_OK
+
+
+def test_fp8_wrappers_refuse():
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    codes = torch.zeros(300, 256, dtype=torch.float8_e4m3fn)
+    scales = torch.ones(3, 2)
+    with pytest.raises(ValueError, match="block_rows must be 1 or 128"):
+        cf.quantize_fp8(x, 64)
+    with pytest.raises(ValueError, match="2-D for square blocks"):
+        cf.quantize_fp8(x.view(2, 2, 256), 128)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        cf.quantize_fp8(x.double())
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        cf.linear_fp8(x, torch.zeros(300, 256, dtype=torch.int8), scales)
+    with pytest.raises(ValueError, match="block scales"):
+        cf.linear_fp8(x, codes, torch.ones(300, 2))
+    with pytest.raises(ValueError, match="block scales"):
+        cf.linear_fp8(x, codes, scales.double())
+    with pytest.raises(ValueError, match="input features"):
+        cf.linear_fp8(x[:, :128], codes, scales)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        cf.linear_fp8(x.float(), codes, scales)
+    a = codes[:4]
+    with pytest.raises(ValueError, match="block scales"):
+        cf.matmul_fp8(a, torch.ones(1, 2), codes, scales)
+    with pytest.raises(ValueError, match="input features"):
+        cf.matmul_fp8(a[:, :128], torch.ones(4, 1), codes, scales)
+    with pytest.raises(ValueError, match="returns float16 or bfloat16"):
+        cf.matmul_fp8(a, torch.ones(4, 2), codes, scales, torch.float32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cf.linear_fp8(x, codes, scales)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cf.quantize_fp8(x)
+
+
+def test_fp8_entry_points_refuse():
+    lib = _abi.load()
+    odd = ctypes.c_void_p(0x1008)
+    q = lambda rows=4, cols=64, br=1, dt=BF16, x=F: lib.cf_quantize_fp8(  # noqa: E731
+        x, dt, F, F, rows, cols, br, None)
+    assert q(rows=-1) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert q(x=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert q(rows=1 << 40, cols=1 << 20) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert q(br=2) == _abi.CF_ERR_UNSUPPORTED
+    assert q(dt=7) == _abi.CF_ERR_UNSUPPORTED
+    assert q(rows=0) == _abi.CF_OK and q(cols=0) == _abi.CF_OK
+    mm = lambda m=4, k=64, n=64, dt=BF16, a=F, y=F: lib.cf_matmul_fp8(  # noqa: E731
+        a, F, F, F, y, m, k, n, dt, None)
+    assert mm(m=-1) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert mm(a=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert mm(m=1 << 31) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert mm(m=1 << 30, n=1 << 30) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert mm(dt=F32) == _abi.CF_ERR_UNSUPPORTED
+    assert mm(k=72) == _abi.CF_ERR_UNSUPPORTED and mm(k=0) == _abi.CF_ERR_UNSUPPORTED
+    assert mm(a=odd) == _abi.CF_ERR_MISALIGNED and mm(y=odd) == _abi.CF_ERR_MISALIGNED
+    assert mm(m=0) == _abi.CF_OK and mm(n=0) == _abi.CF_OK
+    lin = lambda m=40, k=64, x=F, ws=F, size=1 << 20: lib.cf_linear_fp8(  # noqa: E731
+        x, F, F, F, m, k, 64, F16, ws, size, None)
+    need = lib.cf_linear_fp8_workspace_bytes(40, 64)
+    assert need == 40 * 64 + 40 * 4 and lib.cf_linear_fp8_workspace_bytes(8, 64) == 0
+    assert lin(size=need - 1) == _abi.CF_ERR_WORKSPACE
+    assert lin(ws=None) == _abi.CF_ERR_WORKSPACE
+    assert lin(ws=odd) == _abi.CF_ERR_MISALIGNED and lin(x=odd) == _abi.CF_ERR_MISALIGNED
+    assert lin(k=24) == _abi.CF_ERR_UNSUPPORTED
+    assert lin(m=0) == _abi.CF_OK
