@@ -131,7 +131,8 @@ constexpr int kQuantThreads = 256;
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kQuantThreads)
     fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks,
-                             int64_t cols, int64_t row_blocks) {
+                             int64_t cols, int64_t row_blocks, int64_t scale_row,
+                             int64_t scale_kb) {
   constexpr int kUnroll = 4;
   constexpr int kPerCta = kQuantThreads / 16 * kUnroll;
   const int lane16 = threadIdx.x & 15;
@@ -155,7 +156,10 @@ __global__ void __launch_bounds__(kQuantThreads)
     const float s = fp8_scale(m);
     store8<kWide>(codes + at[u], left[u], fp8_codes(f[u], s, __frcp_rn(s), fp8_fast(m, s)));
     const int64_t b = first + u * (kQuantThreads / 16);
-    if (lane16 == 0 && b < blocks) scales[b] = s;
+    if (lane16 == 0 && b < blocks) {
+      const int64_t row = b / row_blocks;
+      scales[row * scale_row + (b - row * row_blocks) * scale_kb] = s;
+    }
   }
 }
 
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 template <typename T>
 int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int64_t cols,
-                 int block_rows, cudaStream_t s) {
+                 int block_rows, bool scales_by_block, cudaStream_t s) {
   const T *in = static_cast<const T *>(x);
   const bool wide = cols % 8 == 0 && aligned_to(x, 16) && aligned_to(codes, 8);
   const int64_t row_blocks = (cols + kBlock - 1) / kBlock;
@@ -205,12 +209,14 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
     const int64_t per_cta = kQuantThreads / 16 * 4;
     const int64_t grid = (blocks + per_cta - 1) / per_cta;
     if (grid > 0x7fffffffll) return CF_ERR_INVALID_ARGUMENT;
+    const int64_t scale_row = scales_by_block ? 1 : row_blocks;
+    const int64_t scale_kb = scales_by_block ? rows : 1;
     if (wide) {
       fp8_quantize_rows_kernel<T, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, row_blocks);
+          in, codes, scales, blocks, cols, row_blocks, scale_row, scale_kb);
     } else {
       fp8_quantize_rows_kernel<T, false><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, row_blocks);
+          in, codes, scales, blocks, cols, row_blocks, scale_row, scale_kb);
     }
     return check_launch();
   }
@@ -232,13 +238,18 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
   return CF_OK;
 }
 
+// scales_by_block: the scales of 1 x 128 blocks as [kb][rows], which is how the
+// products read them, instead of [rows][kb].
 int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, int64_t rows,
-                     int64_t cols, int block_rows, cudaStream_t s) {
+                     int64_t cols, int block_rows, bool scales_by_block, cudaStream_t s) {
   switch (dtype) {
-    case CF_DTYPE_F32: return quantize_fp8<float>(x, codes, scales, rows, cols, block_rows, s);
+    case CF_DTYPE_F32:
+      return quantize_fp8<float>(x, codes, scales, rows, cols, block_rows, scales_by_block, s);
     case CF_DTYPE_BF16:
-      return quantize_fp8<__nv_bfloat16>(x, codes, scales, rows, cols, block_rows, s);
-    default: return quantize_fp8<__half>(x, codes, scales, rows, cols, block_rows, s);
+      return quantize_fp8<__nv_bfloat16>(x, codes, scales, rows, cols, block_rows,
+                                         scales_by_block, s);
+    default:
+      return quantize_fp8<__half>(x, codes, scales, rows, cols, block_rows, scales_by_block, s);
   }
 }
 
@@ -246,7 +257,8 @@ int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, in
 
 struct Fp8Params {
   const uint8_t *a;      // codes [m, k], or the unquantised x of a fused call
-  const float *a_scales; // [m, kb]
+  const float *a_scales; // of row and 128-block (row * scale_row + kb * scale_kb)
+  int64_t scale_row, scale_kb;
   const uint8_t *b;      // codes [n, k]
   const float *b_scales; // [ceil(n / 128), kb]
   void *y;               // [m, n]
@@ -373,8 +385,9 @@ __global__ void __launch_bounds__(kStreamWarps *kWarp)
         xc[0] = cur.x[nt][0];
         xc[1] = cur.x[nt][1];
         const int64_t m = nt * 8 + 2 * t;
-        s0 = m < p.m ? __ldg(p.a_scales + m * p.num_kb + kb) : 0.0f;
-        s1 = m + 1 < p.m ? __ldg(p.a_scales + (m + 1) * p.num_kb + kb) : 0.0f;
+        const float *scale = p.a_scales + kb * p.scale_kb + m * p.scale_row;
+        s0 = m < p.m ? __ldg(scale) : 0.0f;
+        s1 = m + 1 < p.m ? __ldg(scale + p.scale_row) : 0.0f;
       }
       s0 *= ws;
       s1 *= ws;
@@ -442,106 +455,150 @@ int launch_stream(const Fp8Params &p, cudaStream_t s) {
   return check_launch();
 }
 
-// Many rows: 128-token x 256-feature tiles on tcgen05. One MMA group of four
-// (K = 32 each) covers a 128-block of k into one of two TMEM buffers; eight
-// epilogue warps (a thread is a token and half the tile's features) read each
-// finished block, multiply by a_scale b_scale and add into registers while the
-// next block is computed into the other buffer. Half a tile's features are one
-// 128-row block of b, so a thread's scale of a block is one number.
-constexpr int kTileM = 128, kTileN = 256;
-constexpr int kTileThreads = 384;  // warps 0-7 epilogue, 8 producer, 9 MMA, 10-11 idle
-// Registers of an epilogue and of another thread: a share of the 168 that 384
-// threads start with (2 * 216 + 72 = 3 * 168), since an epilogue thread holds
-// 128 fp32 sums.
-constexpr int kTileEpilogueRegs = 216, kTileOtherRegs = 72;
-constexpr int kTileStages = 4;
-constexpr int kTileABytes = kTileM * kBlock;
-constexpr int kTileStageBytes = (kTileM + kTileN) * kBlock;
-constexpr size_t kTileSmem = 1024 + static_cast<size_t>(kTileStages) * kTileStageBytes + 256;
+// Many rows: tiles on tcgen05, 128 tokens a CTA and kN features. One MMA group
+// of four (K = 32 each) covers a 128-block of k into one of several TMEM buffers;
+// sixteen epilogue warps (a thread is a token and a quarter of the tile's
+// features) read each finished block, multiply by a_scale b_scale and add into
+// registers while the next blocks are computed. Reading a block is a chain of
+// barrier, TMEM load and use, several times longer than its share of the MMA's
+// time: sixteen warps overlap four such chains on each scheduler (eight warps of
+// twice the features measured 1300 TFLOP/s at [16384, 8192] x [28672, 8192]).
+// kCtas = 2: CTA pairs, 256 tokens x 256 features, each CTA staging half of b's
+// rows, which halves b's shared-memory traffic for each MMA.
+constexpr int kTileM = 128;
+constexpr int kEpilogueWarps = 16;
+constexpr int kTileThreads = 32 * (kEpilogueWarps + 4);  // + producer, MMA, two idle
+// Registers of an epilogue and of another thread: shares of the 96 that 640
+// threads start with (4 * 112 + 32 = 5 * 96).
+constexpr int kTileEpilogueRegs = 112, kTileOtherRegs = 32;
 
-template <bool kBf16>
+template <int kCtas, int kN>
+struct TileCfg {
+  static constexpr int kBRows = kN / kCtas;
+  static constexpr int kABytes = kTileM * kBlock;
+  static constexpr int kStageBytes = kABytes + kBRows * kBlock;
+  static constexpr int kStages = 196608 / kStageBytes;  // 192 KB of the SM's 227
+  static constexpr int kBuffers = 512 / kN < 4 ? 512 / kN : 4;
+  static constexpr int kTmemCols = kBuffers * kN;
+  static constexpr int kThreadCols = kN / (kEpilogueWarps / 4);
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
+};
+
+// 16 or 32 TMEM columns of a lane, without the wait.
+template <int kCols>
+__device__ __forceinline__ void tmem_columns(uint32_t addr, uint32_t (&v)[32]) {
+  if constexpr (kCols == 16) {
+    ptx::tmem_ld_32x32b_x16(addr, v);
+  } else {
+    ptx::tmem_ld_32x32b_x32(addr, v);
+  }
+}
+
+template <int kCtas, int kN, bool kBf16>
 __global__ void __launch_bounds__(kTileThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
+  using C = TileCfg<kCtas, kN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kTileStages * kTileStageBytes);
-  uint64_t *empty = full + kTileStages;
-  uint64_t *tmem_full = empty + kTileStages;  // [2]
-  uint64_t *tmem_empty = tmem_full + 2;       // [2]
-  uint64_t *drain = tmem_empty + 2;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kStages * C::kStageBytes);
+  uint64_t *empty = full + C::kStages;
+  uint64_t *tmem_full = empty + C::kStages;
+  uint64_t *tmem_empty = tmem_full + C::kBuffers;
+  uint64_t *drain = tmem_empty + C::kBuffers;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
   const int warp = threadIdx.x / kWarp;
   const int lane = threadIdx.x % kWarp;
+  const uint32_t rank = kCtas == 2 ? ptx::cluster_ctarank() : 0;
   const int tiles = p.m_tiles * p.n_tiles;
+  const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kTileStages; ++s) {
+    for (int s = 0; s < C::kStages; ++s) {
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&empty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < C::kBuffers; ++i) {
       ptx::mbar_init(&tmem_full[i], 1);
-      ptx::mbar_init(&tmem_empty[i], 8);
+      ptx::mbar_init(&tmem_empty[i], kCtas * kEpilogueWarps);
     }
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kEpilogueWarps && lane == 0) {
     ptx::prefetch_tensor_map(&tm_a);
     ptx::prefetch_tensor_map(&tm_b);
   }
-  if (warp == 9) {
-    ptx::tmem_alloc(tmem_slot, 512);
-    ptx::tmem_relinquish();
+  if (warp == kEpilogueWarps + 1) {
+    if constexpr (kCtas == 2) {
+      ptx::tmem_alloc_pair(tmem_slot, C::kTmemCols);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, C::kTmemCols);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if constexpr (kCtas == 2) ptx::cluster_sync();  // both CTAs' barriers are ready
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) ptx::lower_registers<kTileOtherRegs>();
-  if (warp == 8) {
+  if (warp >= kEpilogueWarps) ptx::lower_registers<kTileOtherRegs>();
+  if (warp == kEpilogueWarps) {
+    // ------------------------------------------------------------------ producer
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, outstanding = 0, parities = 0;
-      for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+      for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
         int tm, tn;
         band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
+        const int a_row = (tm * kCtas + static_cast<int>(rank)) * kTileM;
+        const int b_row = tn * kN + static_cast<int>(rank) * C::kBRows;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
             record_timeout(p.err, abort_flag);
             break;
           }
-          uint8_t *sa = smem + stage * kTileStageBytes;
-          ptx::mbar_expect_tx(&full[stage], kTileStageBytes);
-          ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, tm * kTileM);
-          ptx::tma_load_2d(sa + kTileABytes, &tm_b, &full[stage], kb * kBlock, tn * kTileN);
+          uint8_t *sa = smem + stage * C::kStageBytes;
+          if constexpr (kCtas == 2) {
+            // The even CTA's barrier counts both CTAs' bytes.
+            const uint32_t bar = ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0);
+            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * C::kStageBytes);
+            ptx::tma_load_2d_pair(sa, &tm_a, bar, kb * kBlock, a_row);
+            ptx::tma_load_2d_pair(sa + C::kABytes, &tm_b, bar, kb * kBlock, b_row);
+          } else {
+            ptx::mbar_expect_tx(&full[stage], C::kStageBytes);
+            ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, a_row);
+            ptx::tma_load_2d(sa + C::kABytes, &tm_b, &full[stage], kb * kBlock, b_row);
+          }
           outstanding |= 1u << stage;
           parities = (parities & ~(1u << stage)) | (phase << stage);
-          if (++stage == kTileStages) {
+          if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      if (aborted(abort_flag)) {
-        for (int s = 0; s < kTileStages; ++s) {
+      if (aborted(abort_flag) && rank == 0) {
+        // Let loads in flight (both CTAs' count here) land before the end.
+        for (int s = 0; s < C::kStages; ++s) {
           if (outstanding & (1u << s)) {
             ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
           }
         }
       }
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t idesc = ptx::make_idesc_e4m3(kTileM, kTileN);
+  } else if (warp == kEpilogueWarps + 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = ptx::make_idesc_e4m3(kTileM * kCtas, kN);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
-      for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+      for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!ptx::mbar_wait(&tmem_empty[buf], buf_phase ^ 1) ||
               !ptx::mbar_wait(&full[stage], phase)) {
@@ -549,75 +606,101 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_addr(smem + stage * kTileStageBytes);
+          const uint32_t sa = ptx::smem_addr(smem + stage * C::kStageBytes);
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            ptx::mma_f8f6f4(tmem + buf * kTileN, kmajor_desc(sa, 128, ks),
-                            kmajor_desc(sa + kTileABytes, 128, ks), idesc, ks > 0);
+            const uint64_t a_desc = kmajor_desc(sa, 128, ks);
+            const uint64_t b_desc = kmajor_desc(sa + C::kABytes, 128, ks);
+            if constexpr (kCtas == 2) {
+              ptx::mma_f8f6f4_pair(tmem + buf * kN, a_desc, b_desc, idesc, ks > 0);
+            } else {
+              ptx::mma_f8f6f4(tmem + buf * kN, a_desc, b_desc, idesc, ks > 0);
+            }
           }
-          ptx::mma_commit(&empty[stage]);
-          ptx::mma_commit(&tmem_full[buf]);
-          if (++stage == kTileStages) {
+          if constexpr (kCtas == 2) {
+            ptx::mma_commit_pair(&empty[stage]);
+            ptx::mma_commit_pair(&tmem_full[buf]);
+          } else {
+            ptx::mma_commit(&empty[stage]);
+            ptx::mma_commit(&tmem_full[buf]);
+          }
+          if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1;
           }
-          if (++buf == 2) {
+          if (++buf == C::kBuffers) {
             buf = 0;
             buf_phase ^= 1;
           }
         }
       }
       if (aborted(abort_flag)) {
-        ptx::mma_commit(drain);
+        if constexpr (kCtas == 2) {
+          ptx::mma_commit_pair(drain);
+        } else {
+          ptx::mma_commit(drain);
+        }
         ptx::mbar_wait(drain, 0, 200000000ull);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < kEpilogueWarps) {
+    // ------------------------------------------------------------------ epilogue
     ptx::raise_registers<kTileEpilogueRegs>();
-    const int quarter = warp % 4, half = warp / 4;
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    constexpr int kCols = C::kThreadCols;
+    constexpr int kChunk = kCols < 32 ? kCols : 32;
+    const int quarter = warp % 4;
+    const int col = warp / 4 * kCols;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col;
+    const uint32_t empty_addr =  // in the CTA that issues the MMAs
+        kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(tmem_empty), 0) : 0;
     int buf = 0;
     uint32_t buf_phase = 0;
-    for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+    for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
       int tm, tn;
       band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
-      const int64_t row = static_cast<int64_t>(tm) * kTileM + quarter * 32 + lane;
-      const int64_t col0 = static_cast<int64_t>(tn) * kTileN + half * 128;
-      const float *a_scale = p.a_scales + (row < p.m ? row : 0) * p.num_kb;
-      const float *b_scale = p.b_scales + (col0 < p.n ? col0 / kBlock : 0) * p.num_kb;
-      uint64_t acc[64];
+      const int row = (tm * kCtas + static_cast<int>(rank)) * kTileM + quarter * 32 + lane;
+      const int col0 = tn * kN + col;
+      // Features of one thread lie in one 128-row block of b.
+      const float *a_scale = p.a_scales + (row < p.m ? row : 0) * p.scale_row;
+      const float *b_scale =
+          p.b_scales + static_cast<int64_t>(col0 < p.n ? col0 / kBlock : 0) * p.num_kb;
+      float acc[kCols];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0;
-      float scale = a_scale[0] * b_scale[0];
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+      float scale = __ldg(a_scale) * __ldg(b_scale);
       bool ok = true;
       for (int kb = 0; kb < p.num_kb; ++kb) {
-        const int ahead = kb + 1 < p.num_kb ? kb + 1 : kb;
-        const float next = __ldg(a_scale + ahead) * __ldg(b_scale + ahead);
-        ok = ptx::warp_wait(&tmem_full[buf], buf_phase);
+        if (kb + 1 < p.num_kb) {
+          a_scale += p.scale_kb;
+          ++b_scale;
+        }
+        const float next_a = __ldg(a_scale), next_b = __ldg(b_scale);
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&tmem_full[buf], buf_phase));
         if (!ok) {
           if (lane == 0) record_timeout(p.err, abort_flag);
           break;
         }
         ptx::tc_fence_after();
-        const uint64_t s2 = ptx::splat_f32x2(scale);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kCols / kChunk; ++c) {
           uint32_t v[32];
-          ptx::tmem_ld_32x32b_x32(t_row + buf * kTileN + c * 32, v);
+          tmem_columns<kChunk>(t_row + buf * kN + c * kChunk, v);
           ptx::tmem_ld_wait();
-          if (c == 3) {
+          if (c == kCols / kChunk - 1) {
             ptx::tc_fence_before();
-            ptx::warp_arrive(&tmem_empty[buf]);
+            if constexpr (kCtas == 2) {
+              ptx::warp_arrive_cluster(empty_addr + buf * 8);
+            } else {
+              ptx::warp_arrive(&tmem_empty[buf]);
+            }
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint64_t d = ptx::pack_f32x2(__uint_as_float(v[2 * e]),
-                                               __uint_as_float(v[2 * e + 1]));
-            acc[c * 16 + e] = ptx::fma_f32x2(s2, d, acc[c * 16 + e]);
+          for (int e = 0; e < kChunk; ++e) {
+            acc[c * kChunk + e] = fmaf(scale, __uint_as_float(v[e]), acc[c * kChunk + e]);
           }
         }
-        scale = next;
-        if (++buf == 2) {
+        scale = next_a * next_b;
+        if (++buf == C::kBuffers) {
           buf = 0;
           buf_phase ^= 1;
         }
@@ -627,12 +710,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         uint16_t *out = static_cast<uint16_t *>(p.y) + row * p.n + col0;
         const bool wide = p.n % 8 == 0;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
+        for (int c = 0; c < kCols / 8; ++c) {
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 f = ptx::unpack_f32x2(acc[c * 4 + e]);
-            w[e] = kBf16 ? ptx::pack_bf16x2(f.x, f.y) : ptx::pack_f16x2(f.x, f.y);
+            const float lo = acc[c * 8 + 2 * e], hi = acc[c * 8 + 2 * e + 1];
+            w[e] = kBf16 ? ptx::pack_bf16x2(lo, hi) : ptx::pack_f16x2(lo, hi);
           }
           if (wide) {
             if (col0 + c * 8 < p.n) {
@@ -653,28 +736,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  // Neither CTA leaves while the other's MMAs or arrivals may still reach it.
+  if constexpr (kCtas == 2) ptx::cluster_sync();
+  if (warp == kEpilogueWarps + 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, 512);
+    if constexpr (kCtas == 2) {
+      ptx::tmem_dealloc_pair(tmem, C::kTmemCols);
+    } else {
+      ptx::tmem_dealloc(tmem, C::kTmemCols);
+    }
   }
 }
 
-template <bool kBf16>
+template <int kCtas, int kN, bool kBf16>
 int launch_tiles(Fp8Params p, cudaStream_t s) {
-  p.m_tiles = static_cast<int>((p.m + kTileM - 1) / kTileM);
-  p.n_tiles = static_cast<int>((p.n + kTileN - 1) / kTileN);
+  using C = TileCfg<kCtas, kN>;
+  p.m_tiles = static_cast<int>((p.m + kCtas * kTileM - 1) / (kCtas * kTileM));
+  p.n_tiles = static_cast<int>((p.n + kN - 1) / kN);
   // As many row blocks of a in a band as stay in L2 while b streams past.
-  const int64_t fit = (int64_t{32} << 20) / (kTileM * std::max<int64_t>(p.k, 1));
+  const int64_t fit = (int64_t{32} << 20) / (kCtas * kTileM * std::max<int64_t>(p.k, 1));
   p.band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, fit)));
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
   CUtensorMap tm_a, tm_b;
   if (int st = make_map(&tm_a, p.a, 1, p.k, p.m, kBlock, kTileM, true)) return st;
-  if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, kTileN, true)) return st;
-  if (int st = allow_dynamic_smem<fp8_tile_kernel<kBf16>>(kTileSmem)) return st;
-  const unsigned grid = static_cast<unsigned>(
-      std::min<int64_t>(static_cast<int64_t>(p.m_tiles) * p.n_tiles, sm_count()));
-  fp8_tile_kernel<kBf16><<<grid, kTileThreads, kTileSmem, s>>>(tm_a, tm_b, p);
+  if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, C::kBRows, true)) return st;
+  if (int st = allow_dynamic_smem<fp8_tile_kernel<kCtas, kN, kBf16>>(C::kSmem)) return st;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16>, tm_a, tm_b, p));
   return check_launch();
 }
 
@@ -683,7 +784,14 @@ int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
   if (p.m <= 8) return launch_stream<T, 1, false>(p, s);
   if (p.m <= 16) return launch_stream<T, 2, false>(p, s);
   if (p.m <= kStreamRows) return launch_stream<T, 4, false>(p, s);
-  return launch_tiles<std::is_same_v<T, __nv_bfloat16>>(p, s);
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  // Pairs of CTAs once their tiles fill most of the GPU; otherwise smaller tiles
+  // for more of them.
+  const int64_t pairs = (p.m + 255) / 256 * ((p.n + 255) / 256);
+  if (pairs * 4 >= sm_count()) return launch_tiles<2, 256, kBf16>(p, s);
+  const int64_t wide = (p.m + 127) / 128 * ((p.n + 127) / 128);
+  if (wide * 4 >= sm_count() * 3) return launch_tiles<1, 128, kBf16>(p, s);
+  return launch_tiles<1, 64, kBf16>(p, s);
 }
 
 int check_fp8_shape(int64_t m, int64_t k, int64_t n, int dtype) {
@@ -691,8 +799,8 @@ int check_fp8_shape(int64_t m, int64_t k, int64_t n, int dtype) {
   if (dtype != CF_DTYPE_BF16 && dtype != CF_DTYPE_F16) return CF_ERR_UNSUPPORTED;
   if (m == 0 || n == 0) return CF_OK;
   if (k == 0 || k % 16 != 0) return CF_ERR_UNSUPPORTED;
-  if (m > 0x7fffffffll - kTileM || n > 0x7fffffffll - kTileN || k > 0x7fffffffll - kBlock ||
-      (m + kTileM - 1) / kTileM * ((n + kTileN - 1) / kTileN) > 0x7fffffffll) {
+  if (m > 0x7fffffffll - 256 || n > 0x7fffffffll - 256 || k > 0x7fffffffll - kBlock ||
+      (m + 127) / 128 * ((n + 63) / 64) > 0x7fffffffll) {
     return CF_ERR_INVALID_ARGUMENT;  // tile counts and coordinates are 32-bit
   }
   return CF_OK;
@@ -710,6 +818,8 @@ Fp8Params fp8_params(const void *a, const float *a_scales, const uint8_t *b, con
   p.n = n;
   p.k = k;
   p.num_kb = static_cast<int>((k + kBlock - 1) / kBlock);
+  p.scale_row = p.num_kb;
+  p.scale_kb = 1;
   return p;
 }
 
@@ -734,7 +844,7 @@ int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
   if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 37)) {
     return CF_ERR_INVALID_ARGUMENT;
   }
-  return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows,
+  return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows, false,
                                reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -780,8 +890,12 @@ int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, 
   if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
   uint8_t *codes = static_cast<uint8_t *>(workspace);
   float *scales = reinterpret_cast<float *>(codes + cfb::fp8_code_bytes(m, k));
-  if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, s)) return st;
-  return cf_matmul_fp8(codes, scales, w_codes, w_scales, y, m, k, n, dtype, stream);
+  if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, true, s)) return st;
+  cfb::Fp8Params p = cfb::fp8_params(codes, scales, w_codes, w_scales, y, m, k, n);
+  p.scale_row = 1;
+  p.scale_kb = m;
+  return dtype == CF_DTYPE_BF16 ? cfb::matmul_fp8<__nv_bfloat16>(p, s)
+                                : cfb::matmul_fp8<__half>(p, s);
 }
 
 }  // extern "C"
