@@ -457,45 +457,41 @@ int launch_stream(const Fp8Params &p, cudaStream_t s) {
 
 // Many rows: tiles on tcgen05, 128 tokens a CTA and kN features. One MMA group
 // of four (K = 32 each) covers a 128-block of k into one of several TMEM buffers;
-// sixteen epilogue warps (a thread is a token and a quarter of the tile's
-// features) read each finished block, multiply by a_scale b_scale and add into
-// registers while the next blocks are computed. Reading a block is a chain of
-// barrier, TMEM load and use, several times longer than its share of the MMA's
-// time: sixteen warps overlap four such chains on each scheduler (eight warps of
-// twice the features measured 1300 TFLOP/s at [16384, 8192] x [28672, 8192]).
-// kCtas = 2: CTA pairs, 256 tokens x 256 features, each CTA staging half of b's
-// rows, which halves b's shared-memory traffic for each MMA.
+// epilogue warps (a thread is a token and kThreadCols of the tile's features)
+// read each finished block, multiply by a_scale b_scale and add into registers
+// while the next blocks are computed.
+//
+// What bounds it is the way from a finished block to a free buffer (barrier,
+// TMEM load, barrier), since TMEM holds two blocks: without an epilogue the MMAs
+// run at 3.0 PFLOP/s at [16384, 8192] x [28672, 8192], with empty epilogues at
+// 2.45. Registers hold half of that: 256 features' sums and one quarter of a
+// block. (192 features, read at once and the buffer freed before any addition,
+// ran 12 % slower: a smaller block takes as long.) kCtas = 2: CTA pairs, 256
+// tokens, each CTA staging half of b's rows.
 constexpr int kTileM = 128;
-constexpr int kEpilogueWarps = 16;
-constexpr int kTileThreads = 32 * (kEpilogueWarps + 4);  // + producer, MMA, two idle
-// Registers of an epilogue and of another thread: shares of the 96 that 640
-// threads start with (4 * 112 + 32 = 5 * 96).
-constexpr int kTileEpilogueRegs = 112, kTileOtherRegs = 32;
 
 template <int kCtas, int kN>
 struct TileCfg {
+  static constexpr int kThreadCols = kN >= 128 ? 64 : 32;
+  static constexpr int kEpilogueWarps = 4 * kN / kThreadCols;
+  static constexpr int kThreads = 32 * (kEpilogueWarps + 4);  // + producer, MMA, two idle
+  // Sixteen epilogue warps: 96 registers a thread at launch, moved to where the
+  // sums are (4 * 112 + 32 = 5 * 96), and columns are read 32 at a time. Fewer
+  // warps have registers enough to read their share at once.
+  static constexpr bool kMoveRegs = kEpilogueWarps == 16;
+  static constexpr int kEpilogueRegs = 112, kOtherRegs = 32;
+  static constexpr int kAtOnce = kMoveRegs ? 32 : kThreadCols;
   static constexpr int kBRows = kN / kCtas;
   static constexpr int kABytes = kTileM * kBlock;
   static constexpr int kStageBytes = kABytes + kBRows * kBlock;
-  static constexpr int kStages = 196608 / kStageBytes;  // 192 KB of the SM's 227
+  static constexpr int kStages = 200704 / kStageBytes;  // 196 KB of the SM's 227
   static constexpr int kBuffers = 512 / kN < 4 ? 512 / kN : 4;
-  static constexpr int kTmemCols = kBuffers * kN;
-  static constexpr int kThreadCols = kN / (kEpilogueWarps / 4);
+  static constexpr int kTmemCols = kBuffers * kN <= 256 ? 256 : 512;
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
 };
 
-// 16 or 32 TMEM columns of a lane, without the wait.
-template <int kCols>
-__device__ __forceinline__ void tmem_columns(uint32_t addr, uint32_t (&v)[32]) {
-  if constexpr (kCols == 16) {
-    ptx::tmem_ld_32x32b_x16(addr, v);
-  } else {
-    ptx::tmem_ld_32x32b_x32(addr, v);
-  }
-}
-
 template <int kCtas, int kN, bool kBf16>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
   using C = TileCfg<kCtas, kN>;
@@ -522,17 +518,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int i = 0; i < C::kBuffers; ++i) {
       ptx::mbar_init(&tmem_full[i], 1);
-      ptx::mbar_init(&tmem_empty[i], kCtas * kEpilogueWarps);
+      ptx::mbar_init(&tmem_empty[i], kCtas * C::kEpilogueWarps);
     }
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == kEpilogueWarps && lane == 0) {
+  if (warp == C::kEpilogueWarps && lane == 0) {
     ptx::prefetch_tensor_map(&tm_a);
     ptx::prefetch_tensor_map(&tm_b);
   }
-  if (warp == kEpilogueWarps + 1) {
+  if (warp == C::kEpilogueWarps + 1) {
     if constexpr (kCtas == 2) {
       ptx::tmem_alloc_pair(tmem_slot, C::kTmemCols);
       ptx::tmem_relinquish_pair();
@@ -547,8 +543,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= kEpilogueWarps) ptx::lower_registers<kTileOtherRegs>();
-  if (warp == kEpilogueWarps) {
+  if constexpr (C::kMoveRegs) {
+    if (warp >= C::kEpilogueWarps) ptx::lower_registers<C::kOtherRegs>();
+  }
+  if (warp == C::kEpilogueWarps) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
       int stage = 0;
@@ -592,10 +590,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
     }
-  } else if (warp == kEpilogueWarps + 1) {
+  } else if (warp == C::kEpilogueWarps + 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop and one lane issues, on descriptors that only
+    // need an addition: this thread's instructions are the pipe's idle time (a
+    // divergent lane building each descriptor took 900 cycles a block).
+    if (rank == 0) {
       const uint32_t idesc = ptx::make_idesc_e4m3(kTileM * kCtas, kN);
+      const uint64_t desc = kmajor_desc(ptx::smem_addr(smem), 128, 0);
+      const bool issuer = ptx::elect_one();
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
@@ -606,24 +609,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_addr(smem + stage * C::kStageBytes);
+          if (issuer) {
+            const uint64_t a_desc = desc + static_cast<uint32_t>(stage * (C::kStageBytes / 16));
+            const uint64_t b_desc = a_desc + C::kABytes / 16;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t a_desc = kmajor_desc(sa, 128, ks);
-            const uint64_t b_desc = kmajor_desc(sa + C::kABytes, 128, ks);
+            for (int ks = 0; ks < 4; ++ks) {  // 32 bytes further in the swizzle atom
+              if constexpr (kCtas == 2) {
+                ptx::mma_f8f6f4_pair(tmem + buf * kN, a_desc + 2 * ks, b_desc + 2 * ks, idesc,
+                                     ks > 0);
+              } else {
+                ptx::mma_f8f6f4(tmem + buf * kN, a_desc + 2 * ks, b_desc + 2 * ks, idesc, ks > 0);
+              }
+            }
             if constexpr (kCtas == 2) {
-              ptx::mma_f8f6f4_pair(tmem + buf * kN, a_desc, b_desc, idesc, ks > 0);
+              ptx::mma_commit_pair(&empty[stage]);
+              ptx::mma_commit_pair(&tmem_full[buf]);
             } else {
-              ptx::mma_f8f6f4(tmem + buf * kN, a_desc, b_desc, idesc, ks > 0);
+              ptx::mma_commit(&empty[stage]);
+              ptx::mma_commit(&tmem_full[buf]);
             }
           }
-          if constexpr (kCtas == 2) {
-            ptx::mma_commit_pair(&empty[stage]);
-            ptx::mma_commit_pair(&tmem_full[buf]);
-          } else {
-            ptx::mma_commit(&empty[stage]);
-            ptx::mma_commit(&tmem_full[buf]);
-          }
+          __syncwarp();
           if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1;
@@ -635,19 +641,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       if (aborted(abort_flag)) {
-        if constexpr (kCtas == 2) {
-          ptx::mma_commit_pair(drain);
-        } else {
-          ptx::mma_commit(drain);
+        if (issuer) {
+          if constexpr (kCtas == 2) {
+            ptx::mma_commit_pair(drain);
+          } else {
+            ptx::mma_commit(drain);
+          }
         }
         ptx::mbar_wait(drain, 0, 200000000ull);
       }
     }
-  } else if (warp < kEpilogueWarps) {
+  } else if (warp < C::kEpilogueWarps) {
     // ------------------------------------------------------------------ epilogue
-    ptx::raise_registers<kTileEpilogueRegs>();
+    if constexpr (C::kMoveRegs) ptx::raise_registers<C::kEpilogueRegs>();
     constexpr int kCols = C::kThreadCols;
-    constexpr int kChunk = kCols < 32 ? kCols : 32;
     const int quarter = warp % 4;
     const int col = warp / 4 * kCols;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col;
@@ -667,26 +674,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
-      float scale = __ldg(a_scale) * __ldg(b_scale);
+      // Scales are loaded two blocks ahead and multiplied when they are used: a
+      // load from L2 outlasts a block's products.
+      float a0 = __ldg(a_scale), b0 = __ldg(b_scale), a1 = 0.0f, b1 = 0.0f;
+      a_scale += p.scale_kb;
+      ++b_scale;
+      if (p.num_kb > 1) {
+        a1 = __ldg(a_scale);
+        b1 = __ldg(b_scale);
+      }
       bool ok = true;
       for (int kb = 0; kb < p.num_kb; ++kb) {
-        if (kb + 1 < p.num_kb) {
-          a_scale += p.scale_kb;
-          ++b_scale;
+        const float scale = a0 * b0;
+        a0 = a1;
+        b0 = b1;
+        a_scale += p.scale_kb;
+        ++b_scale;
+        if (kb + 2 < p.num_kb) {
+          a1 = __ldg(a_scale);
+          b1 = __ldg(b_scale);
         }
-        const float next_a = __ldg(a_scale), next_b = __ldg(b_scale);
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&tmem_full[buf], buf_phase));
+        ok = !__any_sync(0xffffffffu, !ptx::mbar_wait(&tmem_full[buf], buf_phase));
         if (!ok) {
           if (lane == 0) record_timeout(p.err, abort_flag);
           break;
         }
         ptx::tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < kCols / kChunk; ++c) {
-          uint32_t v[32];
-          tmem_columns<kChunk>(t_row + buf * kN + c * kChunk, v);
+        for (int c0 = 0; c0 < kCols; c0 += C::kAtOnce) {
+          uint32_t v[C::kAtOnce / 32][32];
+#pragma unroll
+          for (int c = 0; c < C::kAtOnce / 32; ++c) {
+            ptx::tmem_ld_32x32b_x32(t_row + buf * kN + c0 + c * 32, v[c]);
+          }
           ptx::tmem_ld_wait();
-          if (c == kCols / kChunk - 1) {
+          if (c0 + C::kAtOnce == kCols) {
             ptx::tc_fence_before();
             if constexpr (kCtas == 2) {
               ptx::warp_arrive_cluster(empty_addr + buf * 8);
@@ -695,11 +717,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
 #pragma unroll
-          for (int e = 0; e < kChunk; ++e) {
-            acc[c * kChunk + e] = fmaf(scale, __uint_as_float(v[e]), acc[c * kChunk + e]);
+          for (int e = 0; e < C::kAtOnce; ++e) {
+            acc[c0 + e] = fmaf(scale, __uint_as_float(v[e / 32][e % 32]), acc[c0 + e]);
           }
         }
-        scale = next_a * next_b;
         if (++buf == C::kBuffers) {
           buf = 0;
           buf_phase ^= 1;
@@ -738,7 +759,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   // Neither CTA leaves while the other's MMAs or arrivals may still reach it.
   if constexpr (kCtas == 2) ptx::cluster_sync();
-  if (warp == kEpilogueWarps + 1) {
+  if (warp == C::kEpilogueWarps + 1) {
     ptx::tc_fence_after();
     if constexpr (kCtas == 2) {
       ptx::tmem_dealloc_pair(tmem, C::kTmemCols);
@@ -765,7 +786,7 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -785,13 +806,18 @@ int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
   if (p.m <= 16) return launch_stream<T, 2, false>(p, s);
   if (p.m <= kStreamRows) return launch_stream<T, 4, false>(p, s);
   constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-  // Pairs of CTAs once their tiles fill most of the GPU; otherwise smaller tiles
-  // for more of them.
-  const int64_t pairs = (p.m + 255) / 256 * ((p.n + 255) / 256);
-  if (pairs * 4 >= sm_count()) return launch_tiles<2, 256, kBf16>(p, s);
-  const int64_t wide = (p.m + 127) / 128 * ((p.n + 127) / 128);
-  if (wide * 4 >= sm_count() * 3) return launch_tiles<1, 128, kBf16>(p, s);
-  return launch_tiles<1, 64, kBf16>(p, s);
+  // The form with the least time by waves of tiles: a 128-block of k takes about
+  // 1300 cycles of a pair's 256 x 256 tile, 780 of a 128 x 128 tile and 700 of a
+  // 128 x 64 tile (measured at k = 4096).
+  const int64_t sms = sm_count();
+  auto cost = [&](int64_t tm, int64_t tn, int64_t slots, int64_t cycles) {
+    const int64_t tiles = (p.m + tm - 1) / tm * ((p.n + tn - 1) / tn);
+    return (tiles + slots - 1) / slots * cycles;
+  };
+  const int64_t pair = cost(256, 256, sms / 2, 1300), wide = cost(128, 128, sms, 780),
+                narrow = cost(128, 64, sms, 700);
+  if (pair <= wide && pair <= narrow) return launch_tiles<2, 256, kBf16>(p, s);
+  return wide <= narrow ? launch_tiles<1, 128, kBf16>(p, s) : launch_tiles<1, 64, kBf16>(p, s);
 }
 
 int check_fp8_shape(int64_t m, int64_t k, int64_t n, int dtype) {

@@ -88,6 +88,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
                                           uint64_t limit_ns = 2000000000ull, bool idle = true) {
   const uint32_t addr = smem_addr(bar);
   if (mbar_try_wait(addr, parity)) return true;
+  // The first tries go without the timer: reading it takes longer than most
+  // waits last, and each try ends by itself within kSuspendHintNs.
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    if (idle ? mbar_try_wait_suspend(addr, parity) : mbar_try_wait(addr, parity)) return true;
+  }
   const uint64_t start = global_timer_ns();
   for (uint32_t i = 0;; ++i) {
     if (idle ? mbar_try_wait_suspend(addr, parity) : mbar_try_wait(addr, parity)) return true;
@@ -366,6 +372,17 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
 
 // 32 lanes x 16 columns: thread t gets lane (base+t), 16 columns in r[0..15].
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// 32 lanes x 16 columns into exactly 16 registers.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
