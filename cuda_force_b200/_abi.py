@@ -98,7 +98,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          ctypes.c_float, _int, _p, ctypes.c_size_t, _p],
     ),
     "cf_quantize_fp8": (_int, [_p, _int, _p, _p, _i64, _i64, _int, _p]),
-    "cf_matmul_fp8": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
+    "cf_matmul_fp8": (_int, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
     "cf_linear_fp8_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "cf_linear_fp8": (
         _int, [_p, _p, _p, _p, _i64, _i64, _i64, _int, _p, ctypes.c_size_t, _p]),

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 template <typename T>
 int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int64_t cols,
-                 int block_rows, bool scales_by_block, cudaStream_t s) {
+                 int block_rows, int64_t scale_pitch, cudaStream_t s) {
   const T *in = static_cast<const T *>(x);
   const bool wide = cols % 8 == 0 && aligned_to(x, 16) && aligned_to(codes, 8);
   const int64_t row_blocks = (cols + kBlock - 1) / kBlock;
@@ -209,8 +209,8 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
     const int64_t per_cta = kQuantThreads / 16 * 4;
     const int64_t grid = (blocks + per_cta - 1) / per_cta;
     if (grid > 0x7fffffffll) return CF_ERR_INVALID_ARGUMENT;
-    const int64_t scale_row = scales_by_block ? 1 : row_blocks;
-    const int64_t scale_kb = scales_by_block ? rows : 1;
+    const int64_t scale_row = scale_pitch > 0 ? 1 : row_blocks;
+    const int64_t scale_kb = scale_pitch > 0 ? scale_pitch : 1;
     if (wide) {
       fp8_quantize_rows_kernel<T, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
           in, codes, scales, blocks, cols, row_blocks, scale_row, scale_kb);
@@ -238,18 +238,18 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
   return CF_OK;
 }
 
-// scales_by_block: the scales of 1 x 128 blocks as [kb][rows], which is how the
-// products read them, instead of [rows][kb].
+// scale_pitch > 0: the scales of 1 x 128 blocks as [kb][scale_pitch], which is how
+// the products read them, instead of [rows][kb].
 int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, int64_t rows,
-                     int64_t cols, int block_rows, bool scales_by_block, cudaStream_t s) {
+                     int64_t cols, int block_rows, int64_t scale_pitch, cudaStream_t s) {
   switch (dtype) {
     case CF_DTYPE_F32:
-      return quantize_fp8<float>(x, codes, scales, rows, cols, block_rows, scales_by_block, s);
+      return quantize_fp8<float>(x, codes, scales, rows, cols, block_rows, scale_pitch, s);
     case CF_DTYPE_BF16:
       return quantize_fp8<__nv_bfloat16>(x, codes, scales, rows, cols, block_rows,
-                                         scales_by_block, s);
+                                         scale_pitch, s);
     default:
-      return quantize_fp8<__half>(x, codes, scales, rows, cols, block_rows, scales_by_block, s);
+      return quantize_fp8<__half>(x, codes, scales, rows, cols, block_rows, scale_pitch, s);
   }
 }
 
@@ -257,8 +257,8 @@ int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, in
 
 struct Fp8Params {
   const uint8_t *a;      // codes [m, k], or the unquantised x of a fused call
-  const float *a_scales; // of row and 128-block (row * scale_row + kb * scale_kb)
-  int64_t scale_row, scale_kb;
+  const float *a_scales; // [kb][a_pitch], a row's at its index
+  int64_t a_pitch;
   const uint8_t *b;      // codes [n, k]
   const float *b_scales; // [ceil(n / 128), kb]
   void *y;               // [m, n]
@@ -385,9 +385,9 @@ __global__ void __launch_bounds__(kStreamWarps *kWarp)
         xc[0] = cur.x[nt][0];
         xc[1] = cur.x[nt][1];
         const int64_t m = nt * 8 + 2 * t;
-        const float *scale = p.a_scales + kb * p.scale_kb + m * p.scale_row;
+        const float *scale = p.a_scales + kb * p.a_pitch + m;
         s0 = m < p.m ? __ldg(scale) : 0.0f;
-        s1 = m + 1 < p.m ? __ldg(scale + p.scale_row) : 0.0f;
+        s1 = m + 1 < p.m ? __ldg(scale + 1) : 0.0f;
       }
       s0 *= ws;
       s1 *= ws;
@@ -462,12 +462,15 @@ int launch_stream(const Fp8Params &p, cudaStream_t s) {
 // while the next blocks are computed.
 //
 // What bounds it is the way from a finished block to a free buffer (barrier,
-// TMEM load, barrier), since TMEM holds two blocks: without an epilogue the MMAs
-// run at 3.0 PFLOP/s at [16384, 8192] x [28672, 8192], with empty epilogues at
-// 2.45. Registers hold half of that: 256 features' sums and one quarter of a
-// block. (192 features, read at once and the buffer freed before any addition,
-// ran 12 % slower: a smaller block takes as long.) kCtas = 2: CTA pairs, 256
-// tokens, each CTA staging half of b's rows.
+// TMEM load, additions, barrier), since TMEM holds two blocks and registers hold
+// 256 features' sums and a quarter of a block. At [16384, 8192] x [28672, 8192]
+// the MMAs alone take 2.4 ms (3.2 PFLOP/s), the additions 0.6 ms on top. (192
+// features, read at once and the buffer freed before any addition, were no
+// faster.) So everything else is kept off these warps: the tokens' scales come by
+// TMA with each stage's operands (loading them from global memory cost 0.4 ms),
+// and results leave through shared memory and TMA (row by row from the threads
+// that hold them, 32 rows an instruction, cost 0.25 ms). kCtas = 2: CTA pairs,
+// 256 tokens, each CTA staging half of b's rows.
 constexpr int kTileM = 128;
 
 template <int kCtas, int kN>
@@ -483,22 +486,36 @@ struct TileCfg {
   static constexpr int kAtOnce = kMoveRegs ? 32 : kThreadCols;
   static constexpr int kBRows = kN / kCtas;
   static constexpr int kABytes = kTileM * kBlock;
-  static constexpr int kStageBytes = kABytes + kBRows * kBlock;
-  static constexpr int kStages = 200704 / kStageBytes;  // 196 KB of the SM's 227
+  static constexpr int kOperandBytes = kABytes + kBRows * kBlock;
+  static constexpr int kScaleBytes = kTileM * 4;
+  static constexpr int kOutBytes = 32 * 64;  // a warp's 32 rows x 32 columns on their way out
   static constexpr int kBuffers = 512 / kN < 4 ? 512 / kN : 4;
   static constexpr int kTmemCols = kBuffers * kN <= 256 ? 256 : 512;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
+  static constexpr int kStages = kN == 256 ? 5 : 6;
+  // A stage's scales are read by the epilogue, after its operands' slot is free
+  // again: the producer's next use of a scale slot has to come after that. It
+  // refills operand slot s once the MMAs of kStages blocks ago retired, and those
+  // began once the block kBuffers before them had left its TMEM buffer, scales
+  // read. So this many slots need no barrier of their own.
+  static constexpr int kScaleSlots = kStages + kBuffers;
+  static constexpr int kOutOffset = kStages * kOperandBytes;
+  static constexpr int kScaleOffset = kOutOffset + kEpilogueWarps * kOutBytes;
+  static constexpr int kBarOffset = kScaleOffset + kScaleSlots * kScaleBytes;
+  static constexpr size_t kSmem = 1024 + kBarOffset + 256;
+  static_assert(kSmem <= 232448, "227 KB of shared memory");
 };
 
 template <int kCtas, int kN, bool kBf16>
 __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
-                    const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
+                    const __grid_constant__ CUtensorMap tm_b,
+                    const __grid_constant__ CUtensorMap tm_scale,
+                    const __grid_constant__ CUtensorMap tm_y, const Fp8Params p) {
   using C = TileCfg<kCtas, kN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kStages * C::kStageBytes);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOffset);
   uint64_t *empty = full + C::kStages;
   uint64_t *tmem_full = empty + C::kStages;
   uint64_t *tmem_empty = tmem_full + C::kBuffers;
@@ -527,6 +544,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   if (warp == C::kEpilogueWarps && lane == 0) {
     ptx::prefetch_tensor_map(&tm_a);
     ptx::prefetch_tensor_map(&tm_b);
+    ptx::prefetch_tensor_map(&tm_scale);
   }
   if (warp == C::kEpilogueWarps + 1) {
     if constexpr (kCtas == 2) {
@@ -549,7 +567,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   if (warp == C::kEpilogueWarps) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      int stage = 0;
+      int stage = 0, slot = 0;
       uint32_t phase = 0, outstanding = 0, parities = 0;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
         int tm, tn;
@@ -561,20 +579,25 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
             record_timeout(p.err, abort_flag);
             break;
           }
-          uint8_t *sa = smem + stage * C::kStageBytes;
+          uint8_t *sa = smem + stage * C::kOperandBytes;
+          uint8_t *scale = smem + C::kScaleOffset + slot * C::kScaleBytes;
+          constexpr uint32_t kBytes = C::kOperandBytes + C::kScaleBytes;
           if constexpr (kCtas == 2) {
             // The even CTA's barrier counts both CTAs' bytes.
             const uint32_t bar = ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0);
-            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * C::kStageBytes);
+            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * kBytes);
             ptx::tma_load_2d_pair(sa, &tm_a, bar, kb * kBlock, a_row);
             ptx::tma_load_2d_pair(sa + C::kABytes, &tm_b, bar, kb * kBlock, b_row);
+            ptx::tma_load_2d_pair(scale, &tm_scale, bar, a_row, kb);
           } else {
-            ptx::mbar_expect_tx(&full[stage], C::kStageBytes);
+            ptx::mbar_expect_tx(&full[stage], kBytes);
             ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, a_row);
             ptx::tma_load_2d(sa + C::kABytes, &tm_b, &full[stage], kb * kBlock, b_row);
+            ptx::tma_load_2d(scale, &tm_scale, &full[stage], a_row, kb);
           }
           outstanding |= 1u << stage;
           parities = (parities & ~(1u << stage)) | (phase << stage);
+          if (++slot == C::kScaleSlots) slot = 0;
           if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1;
@@ -610,7 +633,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
           }
           ptx::tc_fence_after();
           if (issuer) {
-            const uint64_t a_desc = desc + static_cast<uint32_t>(stage * (C::kStageBytes / 16));
+            const uint64_t a_desc = desc + static_cast<uint32_t>(stage * (C::kOperandBytes / 16));
             const uint64_t b_desc = a_desc + C::kABytes / 16;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {  // 32 bytes further in the swizzle atom
@@ -660,39 +683,29 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col;
     const uint32_t empty_addr =  // in the CTA that issues the MMAs
         kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(tmem_empty), 0) : 0;
+    const uint32_t base = ptx::smem_addr(smem);
+    const uint32_t scale0 = base + C::kScaleOffset + (quarter * 32 + lane) * 4;
+    uint32_t scale_addr = scale0;
     int buf = 0;
     uint32_t buf_phase = 0;
     for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
       int tm, tn;
       band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
-      const int row = (tm * kCtas + static_cast<int>(rank)) * kTileM + quarter * 32 + lane;
+      const int row0 = (tm * kCtas + static_cast<int>(rank)) * kTileM + quarter * 32;
       const int col0 = tn * kN + col;
-      // Features of one thread lie in one 128-row block of b.
-      const float *a_scale = p.a_scales + (row < p.m ? row : 0) * p.scale_row;
+      // Features of one thread lie in one 128-row block of b; each lane holds the
+      // scale of one of the next 32 blocks of k.
       const float *b_scale =
           p.b_scales + static_cast<int64_t>(col0 < p.n ? col0 / kBlock : 0) * p.num_kb;
+      float b_next = lane < p.num_kb ? __ldg(b_scale + lane) : 0.0f, b_lane = 0.0f;
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
-      // Scales are loaded two blocks ahead and multiplied when they are used: a
-      // load from L2 outlasts a block's products.
-      float a0 = __ldg(a_scale), b0 = __ldg(b_scale), a1 = 0.0f, b1 = 0.0f;
-      a_scale += p.scale_kb;
-      ++b_scale;
-      if (p.num_kb > 1) {
-        a1 = __ldg(a_scale);
-        b1 = __ldg(b_scale);
-      }
       bool ok = true;
       for (int kb = 0; kb < p.num_kb; ++kb) {
-        const float scale = a0 * b0;
-        a0 = a1;
-        b0 = b1;
-        a_scale += p.scale_kb;
-        ++b_scale;
-        if (kb + 2 < p.num_kb) {
-          a1 = __ldg(a_scale);
-          b1 = __ldg(b_scale);
+        if ((kb & 31) == 0) {
+          b_lane = b_next;
+          if (kb + 32 + lane < p.num_kb) b_next = __ldg(b_scale + kb + 32 + lane);
         }
         ok = !__any_sync(0xffffffffu, !ptx::mbar_wait(&tmem_full[buf], buf_phase));
         if (!ok) {
@@ -700,6 +713,11 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
           break;
         }
         ptx::tc_fence_after();
+        // The scales landed before the MMAs began, which this barrier follows.
+        const float scale =
+            ptx::ld_shared_f32(scale_addr) * __shfl_sync(0xffffffffu, b_lane, kb & 31);
+        scale_addr += C::kScaleBytes;
+        if (scale_addr == scale0 + C::kScaleSlots * C::kScaleBytes) scale_addr = scale0;
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += C::kAtOnce) {
           uint32_t v[C::kAtOnce / 32][32];
@@ -727,32 +745,44 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
         }
       }
       if (!ok) break;
-      if (row < p.m) {
-        uint16_t *out = static_cast<uint16_t *>(p.y) + row * p.n + col0;
-        const bool wide = p.n % 8 == 0;
+      if (p.n % 8 == 0) {
+        // 32 columns at a time through this warp's buffer (64-byte rows, 16-byte
+        // chunks swizzled as the tensor map expects, which spreads the banks).
+        const uint32_t out = base + C::kOutOffset + warp * C::kOutBytes;
 #pragma unroll
-        for (int c = 0; c < kCols / 8; ++c) {
-          uint32_t w[4];
+        for (int c0 = 0; c0 < kCols; c0 += 32) {
+          if (lane == 0) ptx::bulk_wait_read<0>();
+          __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lo = acc[c * 8 + 2 * e], hi = acc[c * 8 + 2 * e + 1];
-            w[e] = kBf16 ? ptx::pack_bf16x2(lo, hi) : ptx::pack_f16x2(lo, hi);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float lo = acc[c0 + c * 8 + 2 * e], hi = acc[c0 + c * 8 + 2 * e + 1];
+              w[e] = kBf16 ? ptx::pack_bf16x2(lo, hi) : ptx::pack_f16x2(lo, hi);
+            }
+            ptx::st_shared_v4(out + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4),
+                              make_uint4(w[0], w[1], w[2], w[3]));
           }
-          if (wide) {
-            if (col0 + c * 8 < p.n) {
-              *reinterpret_cast<uint4 *>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.m && col0 + c0 < p.n) {
+            ptx::tma_store_2d_addr(&tm_y, out, col0 + c0, row0);
+            ptx::bulk_commit();
+          }
+        }
+      } else if (row0 + lane < p.m) {
+        uint16_t *out = static_cast<uint16_t *>(p.y) + (row0 + lane) * p.n + col0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (col0 + c * 8 + e < p.n) {
-                out[c * 8 + e] = static_cast<uint16_t>(w[e / 2] >> (e % 2 * 16));
-              }
-            }
+        for (int e = 0; e < kCols; ++e) {
+          if (col0 + e < p.n) {
+            out[e] = static_cast<uint16_t>(kBf16 ? ptx::pack_bf16x2(acc[e], 0.0f)
+                                                 : ptx::pack_f16x2(acc[e], 0.0f));
           }
         }
       }
     }
+    if (lane == 0) ptx::bulk_wait_all();
   }
 
   ptx::tc_fence_before();
@@ -779,9 +809,17 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   p.band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, fit)));
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
-  CUtensorMap tm_a, tm_b;
+  CUtensorMap tm_a, tm_b, tm_scale, tm_y;
   if (int st = make_map(&tm_a, p.a, 1, p.k, p.m, kBlock, kTileM, true)) return st;
   if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, C::kBRows, true)) return st;
+  if (int st = make_map(&tm_scale, p.a_scales, 4, p.m, p.num_kb, kTileM, 1, false, p.a_pitch)) {
+    return st;
+  }
+  if (p.n % 8 == 0) {  // rows of whole 16-byte units; other results are stored element by element
+    if (int st = make_map(&tm_y, p.y, 2, p.n, p.m, 32, 32, true)) return st;
+  } else {
+    tm_y = tm_a;
+  }
   if (int st = allow_dynamic_smem<fp8_tile_kernel<kCtas, kN, kBf16>>(C::kSmem)) return st;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   cudaLaunchConfig_t cfg = {};
@@ -796,7 +834,8 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16>, tm_a, tm_b, p));
+  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16>, tm_a, tm_b, tm_scale,
+                                  tm_y, p));
   return check_launch();
 }
 
@@ -832,8 +871,8 @@ int check_fp8_shape(int64_t m, int64_t k, int64_t n, int dtype) {
   return CF_OK;
 }
 
-Fp8Params fp8_params(const void *a, const float *a_scales, const uint8_t *b, const float *b_scales,
-                     void *y, int64_t m, int64_t k, int64_t n) {
+Fp8Params fp8_params(const void *a, const float *a_scales, int64_t a_pitch, const uint8_t *b,
+                     const float *b_scales, void *y, int64_t m, int64_t k, int64_t n) {
   Fp8Params p{};
   p.a = static_cast<const uint8_t *>(a);
   p.a_scales = a_scales;
@@ -844,10 +883,11 @@ Fp8Params fp8_params(const void *a, const float *a_scales, const uint8_t *b, con
   p.n = n;
   p.k = k;
   p.num_kb = static_cast<int>((k + kBlock - 1) / kBlock);
-  p.scale_row = p.num_kb;
-  p.scale_kb = 1;
+  p.a_pitch = a_pitch;
   return p;
 }
+
+int64_t fp8_scale_pitch(int64_t m) { return (m + 3) / 4 * 4; }
 
 size_t fp8_code_bytes(int64_t m, int64_t k) {
   return (static_cast<size_t>(m) * static_cast<size_t>(k) + 255) & ~static_cast<size_t>(255);
@@ -870,20 +910,23 @@ int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
   if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 37)) {
     return CF_ERR_INVALID_ARGUMENT;
   }
-  return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows, false,
+  return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows, 0,
                                reinterpret_cast<cudaStream_t>(stream));
 }
 
-int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, const uint8_t *b_codes,
-                  const float *b_scales, void *y, int64_t m, int64_t k, int64_t n, int dtype,
-                  cf_stream_t stream) {
+int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, int64_t a_scale_pitch,
+                  const uint8_t *b_codes, const float *b_scales, void *y, int64_t m, int64_t k,
+                  int64_t n, int dtype, cf_stream_t stream) {
   if (int st = cfb::check_fp8_shape(m, k, n, dtype)) return st;
   if (m == 0 || n == 0) return CF_OK;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !y) return CF_ERR_INVALID_ARGUMENT;
-  if (!cfb::aligned_to(a_codes, 16) || !cfb::aligned_to(b_codes, 16) || !cfb::aligned_to(y, 16)) {
+  if (a_scale_pitch < m) return CF_ERR_INVALID_ARGUMENT;
+  if (a_scale_pitch % 4 != 0) return CF_ERR_UNSUPPORTED;
+  if (!cfb::aligned_to(a_codes, 16) || !cfb::aligned_to(a_scales, 16) ||
+      !cfb::aligned_to(b_codes, 16) || !cfb::aligned_to(y, 16)) {
     return CF_ERR_MISALIGNED;
   }
-  const cfb::Fp8Params p = cfb::fp8_params(a_codes, a_scales, b_codes, b_scales, y, m, k, n);
+  const cfb::Fp8Params p = cfb::fp8_params(a_codes, a_scales, a_scale_pitch, b_codes, b_scales, y, m, k, n);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == CF_DTYPE_BF16 ? cfb::matmul_fp8<__nv_bfloat16>(p, s)
                                 : cfb::matmul_fp8<__half>(p, s);
@@ -891,7 +934,7 @@ int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, const uint8_t *
 
 size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k) {
   if (m <= cfb::kFusedRows || k <= 0) return 0;
-  const int64_t blocks = m * ((k + cfb::kBlock - 1) / cfb::kBlock);
+  const int64_t blocks = cfb::fp8_scale_pitch(m) * ((k + cfb::kBlock - 1) / cfb::kBlock);
   return cfb::fp8_code_bytes(m, k) + static_cast<size_t>(blocks) * sizeof(float);
 }
 
@@ -906,7 +949,7 @@ int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, 
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (m <= cfb::kFusedRows) {
-    const cfb::Fp8Params p = cfb::fp8_params(x, nullptr, w_codes, w_scales, y, m, k, n);
+    const cfb::Fp8Params p = cfb::fp8_params(x, nullptr, 0, w_codes, w_scales, y, m, k, n);
     return dtype == CF_DTYPE_BF16 ? cfb::launch_stream<__nv_bfloat16, 1, true>(p, s)
                                   : cfb::launch_stream<__half, 1, true>(p, s);
   }
@@ -916,10 +959,9 @@ int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, 
   if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
   uint8_t *codes = static_cast<uint8_t *>(workspace);
   float *scales = reinterpret_cast<float *>(codes + cfb::fp8_code_bytes(m, k));
-  if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, true, s)) return st;
-  cfb::Fp8Params p = cfb::fp8_params(codes, scales, w_codes, w_scales, y, m, k, n);
-  p.scale_row = 1;
-  p.scale_kb = m;
+  const int64_t pitch = cfb::fp8_scale_pitch(m);
+  if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, pitch, s)) return st;
+  const cfb::Fp8Params p = cfb::fp8_params(codes, scales, pitch, w_codes, w_scales, y, m, k, n);
   return dtype == CF_DTYPE_BF16 ? cfb::matmul_fp8<__nv_bfloat16>(p, s)
                                 : cfb::matmul_fp8<__half>(p, s);
 }

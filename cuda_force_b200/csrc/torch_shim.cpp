@@ -604,7 +604,12 @@ at::Tensor matmul_fp8_cuda(const at::Tensor &a_codes, const at::Tensor &a_scales
   const int64_t kp = (k + 15) / 16 * 16;
   const at::Tensor a = aligned16(padded_codes(a_codes, kp));
   const at::Tensor b = aligned16(padded_codes(b_codes, kp));
-  check_status(cf_matmul_fp8(code_ptr(a), a_scales.data_ptr<float>(), code_ptr(b),
+  // The kernels take a's scales by block.
+  const int64_t pitch = (m + 3) / 4 * 4;
+  at::Tensor by_block =
+      at::empty({(k + CF_FP8_BLOCK_SIZE - 1) / CF_FP8_BLOCK_SIZE, pitch}, a_scales.options());
+  by_block.narrow(1, 0, m).copy_(a_scales.view({m, by_block.size(0)}).t());
+  check_status(cf_matmul_fp8(code_ptr(a), by_block.data_ptr<float>(), pitch, code_ptr(b),
                              b_scales.data_ptr<float>(), y.data_ptr(), m, kp, n,
                              dtype == at::kBFloat16 ? CF_DTYPE_BF16 : CF_DTYPE_F16,
                              current_stream()),

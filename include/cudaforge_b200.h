@@ -345,15 +345,16 @@ CF_API int cf_gated_residual_rmsnorm_backward(
 CF_API int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
                            int64_t rows, int64_t cols, int block_rows, cf_stream_t stream);
 
-/* y[m, n] = sum_k a[m, k] b[n, k] with a in blocks of 1 x 128 (a_scales float
- * [m][ceil(k / 128)]) and b in blocks of 128 x 128 (b_scales float
- * [ceil(n / 128)][ceil(k / 128)]), as cf_quantize_fp8 makes them; products of
- * codes are summed over each block in fp32 and scaled in fp32; y is of dtype
- * (f16 or bf16). Requirements: k a positive multiple of 16, codes and y 16-byte
- * aligned. No counterpart in the reference. */
-CF_API int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, const uint8_t *b_codes,
-                         const float *b_scales, void *y, int64_t m, int64_t k, int64_t n,
-                         int dtype, cf_stream_t stream);
+/* y[m, n] = sum_k a[m, k] b[n, k] with a in blocks of 1 x 128 and b in blocks of
+ * 128 x 128 (b_scales float [ceil(n / 128)][ceil(k / 128)]), as cf_quantize_fp8
+ * makes them, except that a's scales are given by block: float
+ * [ceil(k / 128)][a_scale_pitch], row m's at index m. Products of codes are
+ * summed over each block in fp32 and scaled in fp32; y is of dtype (f16 or bf16).
+ * Requirements: k a positive multiple of 16, a_scale_pitch >= m a multiple of 4,
+ * codes, a_scales and y 16-byte aligned. No counterpart in the reference. */
+CF_API int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, int64_t a_scale_pitch,
+                         const uint8_t *b_codes, const float *b_scales, void *y, int64_t m,
+                         int64_t k, int64_t n, int dtype, cf_stream_t stream);
 
 /* cf_quantize_fp8 of x [m, k] (dtype f16 or bf16) in blocks of 1 x 128, then
  * cf_matmul_fp8 with the weight w [n, k] (nn.Linear layout). Up to 8 rows are

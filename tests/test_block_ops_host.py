@@ -116,8 +116,9 @@ def test_fp8_entry_points_refuse():
     assert q(br=2) == _abi.CF_ERR_UNSUPPORTED
     assert q(dt=7) == _abi.CF_ERR_UNSUPPORTED
     assert q(rows=0) == _abi.CF_OK and q(cols=0) == _abi.CF_OK
-    mm = lambda m=4, k=64, n=64, dt=BF16, a=F, y=F: lib.cf_matmul_fp8(  # noqa: E731
-        a, F, F, F, y, m, k, n, dt, None)
+    mm = lambda m=4, k=64, n=64, dt=BF16, a=F, y=F, sc=F, pitch=None: (  # noqa: E731
+        lib.cf_matmul_fp8(a, sc, m + -m % 4 if pitch is None else pitch, F, F, y, m, k, n, dt,
+                          None))
     assert mm(m=-1) == _abi.CF_ERR_INVALID_ARGUMENT
     assert mm(a=None) == _abi.CF_ERR_INVALID_ARGUMENT
     assert mm(m=1 << 31) == _abi.CF_ERR_INVALID_ARGUMENT
@@ -125,6 +126,9 @@ def test_fp8_entry_points_refuse():
     assert mm(dt=F32) == _abi.CF_ERR_UNSUPPORTED
     assert mm(k=72) == _abi.CF_ERR_UNSUPPORTED and mm(k=0) == _abi.CF_ERR_UNSUPPORTED
     assert mm(a=odd) == _abi.CF_ERR_MISALIGNED and mm(y=odd) == _abi.CF_ERR_MISALIGNED
+    assert mm(sc=odd) == _abi.CF_ERR_MISALIGNED
+    assert mm(pitch=3) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert mm(pitch=6) == _abi.CF_ERR_UNSUPPORTED
     assert mm(m=0) == _abi.CF_OK and mm(n=0) == _abi.CF_OK
     lin = lambda m=40, k=64, x=F, ws=F, size=1 << 20: lib.cf_linear_fp8(  # noqa: E731
         x, F, F, F, m, k, 64, F16, ws, size, None)
