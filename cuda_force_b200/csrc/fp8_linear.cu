@@ -41,38 +41,33 @@ __device__ __forceinline__ bool fp8_fast(unsigned absmax_bits, float s) {
   return absmax_bits < 0x7f800000u && s >= 0x1p-60f && s <= 0x1p100f;
 }
 
-// fl32(x / s) without a division: r = fl32(1 / s), q0 = fl(x r), the exact
-// residual and Markstein's correction step (as quant_math.cuh).
-__device__ __forceinline__ float fp8_quotient(float x, float s, float r) {
-  const float q0 = __fmul_rn(x, r);
-  return __fmaf_rn(__fmaf_rn(-q0, s, x), r, q0);
-}
-
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
-// Eight elements to eight codes.
+// Eight elements to eight codes. fl32(x / s) without a division, two at a time: r
+// = fl32(1 / s), q0 = fl(x r), the exact residual and Markstein's correction step
+// (as quant_math.cuh).
 __device__ __forceinline__ uint2 fp8_codes(const float (&f)[8], float s, float r, bool fast) {
   float q[8];
   if (fast) {
+    const uint64_t r2 = ptx::splat_f32x2(r), neg_s2 = ptx::splat_f32x2(-s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = fp8_quotient(f[i], s, r);
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t x2 = ptx::pack_f32x2(f[2 * i], f[2 * i + 1]);
+      const uint64_t q0 = ptx::mul_f32x2(x2, r2);
+      const float2 v = ptx::unpack_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(q0, neg_s2, x2), r2, q0));
+      q[2 * i] = v.x;
+      q[2 * i + 1] = v.y;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(f[i], s);
   }
   return make_uint2(e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16,
                     e4m3x2(q[4], q[5]) | e4m3x2(q[6], q[7]) << 16);
-}
-
-__device__ __forceinline__ unsigned absmax_bits(const float (&f)[8]) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
 }
 
 template <typename T>
@@ -86,30 +81,81 @@ __device__ __forceinline__ float as_float(T v) {
   }
 }
 
-// Eight consecutive elements from p, `left` of them inside the row (the rest
-// are zeros). kWide: p is on a 16-byte boundary and left is 0 or at least 8.
-template <typename T, bool kWide>
-__device__ __forceinline__ void load8(const T *p, int64_t left, float (&f)[8]) {
-  if constexpr (kWide) {
-    if (left <= 0) {
+// Eight consecutive elements as they are stored, and their absmax's bit pattern
+// as an fp32 number (magnitudes of one type order as their bits do, a NaN's
+// highest). 16-bit elements stay packed: two a compare.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.0f;
-    } else if constexpr (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-      const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-      f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+
+  // `left` of the eight are inside the row, the rest are zeros. kWide: p is on a
+  // 16-byte boundary and left is not between 0 and 8.
+  template <bool kWide>
+  __device__ __forceinline__ void load(const T *p, int64_t left) {
+    zero();
+    if constexpr (kWide) {
+      if (left <= 0) return;
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
     } else {
-      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-      const T *e = reinterpret_cast<const T *>(&v);
+      T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < left) e[i] = p[i];
+      }
+    }
+  }
+
+  // Largest magnitude, packed: the bits of one fp32, or of two 16-bit halves.
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) m = larger(m, w[i] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu));
+    return m;
+  }
+
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
+  }
+
+  static __device__ __forceinline__ unsigned bits(uint32_t top) {
+    if constexpr (sizeof(T) == 4) {
+      return top;
+    } else {
+      const uint16_t h = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+      return __float_as_uint(as_float<T>(*reinterpret_cast<const T *>(&h)));
+    }
+  }
+
+  __device__ __forceinline__ void widen(float (&f)[8]) const {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = as_float<T>(e[i]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? as_float<T>(p[i]) : 0.0f;
   }
-}
+
+  __device__ __forceinline__ uint2 codes(float s, float r, bool fast) const {
+    float f[8];
+    widen(f);
+    return fp8_codes(f, s, r, fast);
+  }
+};
 
 template <bool kWide>
 __device__ __forceinline__ void store8(uint8_t *p, int64_t left, uint2 codes) {
@@ -131,35 +177,54 @@ constexpr int kQuantThreads = 256;
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kQuantThreads)
     fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks,
-                             int64_t cols, int64_t row_blocks, int64_t scale_row,
-                             int64_t scale_kb) {
+                             int64_t cols, int row_blocks, int64_t scale_row, int64_t scale_kb) {
   constexpr int kUnroll = 4;
-  constexpr int kPerCta = kQuantThreads / 16 * kUnroll;
+  constexpr int kStride = kQuantThreads / 16;
+  ptx::grid_dep_launch_dependents();  // a product may fetch its weights meanwhile
   const int lane16 = threadIdx.x & 15;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kPerCta + threadIdx.x / 16;
-  float f[kUnroll][8];
-  int64_t at[kUnroll], left[kUnroll];
+  // One division for each CTA; its blocks follow from the first by addition.
+  const int64_t cta_first = static_cast<int64_t>(blockIdx.x) * (kStride * kUnroll);
+  int64_t row = blocks <= 0xffffffffll
+                    ? static_cast<uint32_t>(cta_first) / static_cast<uint32_t>(row_blocks)
+                    : cta_first / row_blocks;
+  int kb = static_cast<int>(cta_first - row * row_blocks) + threadIdx.x / 16;
+  Eight<T> v[kUnroll];
+  int64_t at[kUnroll], left[kUnroll], scale_at[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t b = first + u * (kQuantThreads / 16);
-    const int64_t row = b / row_blocks;
-    const int64_t c = (b - row * row_blocks) * kBlock + lane16 * 8;
-    at[u] = row * cols + c;
-    left[u] = b < blocks ? cols - c : 0;
-    load8<T, kWide>(x + at[u], left[u], f[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    unsigned m = absmax_bits(f[u]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = fp8_scale(m);
-    store8<kWide>(codes + at[u], left[u], fp8_codes(f[u], s, __frcp_rn(s), fp8_fast(m, s)));
-    const int64_t b = first + u * (kQuantThreads / 16);
-    if (lane16 == 0 && b < blocks) {
-      const int64_t row = b / row_blocks;
-      scales[row * scale_row + (b - row * row_blocks) * scale_kb] = s;
+    while (kb >= row_blocks) {
+      kb -= row_blocks;
+      ++row;
     }
+    const int c = kb * kBlock + lane16 * 8;
+    at[u] = row * cols + c;
+    scale_at[u] = row * scale_row + kb * scale_kb;
+    left[u] = cta_first + u * kStride + threadIdx.x / 16 < blocks ? cols - c : -1;
+    v[u].template load<kWide>(x + at[u], left[u]);
+    // -1: no such block; 0: a lane behind the end of a row's last block.
+    left[u] = left[u] < -1 ? 0 : left[u];
+    kb += kStride;
+  }
+  // Each lane divides for one of its half-warp's blocks, not for all of them.
+  uint32_t mine = 0;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    uint32_t top = v[u].top();
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      top = Eight<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if ((lane16 & (kUnroll - 1)) == u) mine = top;
+  }
+  const unsigned m = Eight<T>::bits(mine);
+  const float my_scale = fp8_scale(m);
+  const float my_inverse = fp8_fast(m, my_scale) ? __frcp_rn(my_scale) : 0.0f;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const float s = __shfl_sync(0xffffffffu, my_scale, u, 16);
+    const float r = __shfl_sync(0xffffffffu, my_inverse, u, 16);
+    store8<kWide>(codes + at[u], left[u], v[u].codes(s, r, r != 0.0f));
+    if (lane16 == 0 && left[u] > 0) scales[scale_at[u]] = s;
   }
 }
 
@@ -170,30 +235,34 @@ __global__ void __launch_bounds__(kQuantThreads)
                                int64_t cols) {
   constexpr int kRowsAtOnce = kQuantThreads / 16;
   constexpr int kSteps = kBlock / kRowsAtOnce;
-  __shared__ unsigned warp_max[kQuantThreads / kWarp];
+  __shared__ uint32_t warp_top[kQuantThreads / kWarp];
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kBlock + (threadIdx.x & 15) * 8;
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock + threadIdx.x / 16;
-  float f[kSteps][8];
-  unsigned m = 0;
+  Eight<T> v[kSteps];
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int64_t r = r0 + i * kRowsAtOnce;
-    load8<T, kWide>(x + r * cols + c, r < rows ? cols - c : 0, f[i]);
+    v[i].template load<kWide>(x + r * cols + c, r < rows ? cols - c : 0);
   }
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) m = max(m, absmax_bits(f[i]));
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & (kWarp - 1)) == 0) warp_max[threadIdx.x / kWarp] = m;
+  for (int i = 0; i < kSteps; ++i) top = Eight<T>::larger(top, v[i].top());
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = Eight<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if ((threadIdx.x & (kWarp - 1)) == 0) warp_top[threadIdx.x / kWarp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kQuantThreads / kWarp; ++w) m = max(m, warp_max[w]);
+  for (int w = 0; w < kQuantThreads / kWarp; ++w) top = Eight<T>::larger(top, warp_top[w]);
+  const unsigned m = Eight<T>::bits(top);
   const float s = fp8_scale(m);
   const float inv = __frcp_rn(s);
   const bool fast = fp8_fast(m, s);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int64_t r = r0 + i * kRowsAtOnce;
-    store8<kWide>(codes + r * cols + c, r < rows ? cols - c : 0, fp8_codes(f[i], s, inv, fast));
+    store8<kWide>(codes + r * cols + c, r < rows ? cols - c : 0, v[i].codes(s, inv, fast));
   }
   if (threadIdx.x == 0) scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
 }
@@ -213,10 +282,10 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
     const int64_t scale_kb = scale_pitch > 0 ? scale_pitch : 1;
     if (wide) {
       fp8_quantize_rows_kernel<T, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, row_blocks, scale_row, scale_kb);
+          in, codes, scales, blocks, cols, static_cast<int>(row_blocks), scale_row, scale_kb);
     } else {
       fp8_quantize_rows_kernel<T, false><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, row_blocks, scale_row, scale_kb);
+          in, codes, scales, blocks, cols, static_cast<int>(row_blocks), scale_row, scale_kb);
     }
     return check_launch();
   }
@@ -256,7 +325,7 @@ int quantize_fp8_any(const void *x, int dtype, uint8_t *codes, float *scales, in
 // ---------------------------------------------------------------- products
 
 struct Fp8Params {
-  const uint8_t *a;      // codes [m, k], or the unquantised x of a fused call
+  const uint8_t *a;      // codes [m, k]
   const float *a_scales; // [kb][a_pitch], a row's at its index
   int64_t a_pitch;
   const uint8_t *b;      // codes [n, k]
@@ -265,32 +334,34 @@ struct Fp8Params {
   int64_t m, n, k;
   int num_kb;
   int m_tiles, n_tiles, band;
+  bool after_quantise;  // a's codes come from the kernel launched just before
   unsigned *err;
 };
 
-// Few rows: bound by reading b once. Each warp takes every kWarps-th 128-block of
-// k of 16 * kMT features and multiplies them with all tokens on the warp-wide
+// Few rows: bound by reading b once. Persistent CTAs walk over tiles of 16
+// features; a producer warp streams a tile's rows through a 12-stage ring by TMA
+// (192 KB in flight on an SM; registers held too little of it: 24 us at [8, 4096]
+// x [11008, 4096] with loads straight into fragments), 8 blocks of 128 bytes of k
+// a stage, one for each of eight consumer warps. They multiply on the warp-wide
 // MMA (m16n8k32, features as M, tokens as N): at these shapes the tensor core's
-// rate does not matter, and the operands go straight from global memory to
-// registers, next block in flight. A lane's four fragment words of a feature are
-// 16 consecutive bytes: within a block any order of k will do as long as both
-// operands use it. kQuant quantises the tokens on the way (every CTA again,
-// which eight tokens are few enough for), so the call is one launch.
+// rate does not matter. A lane's fragment words of a feature are 32 consecutive
+// bytes: within a block any order of k will do as long as both operands use it.
+// The warps' sums of a tile meet in shared memory.
 constexpr int kStreamWarps = 8;
+constexpr int kStreamFeatures = 16;
+constexpr int kStreamStages = 12;
+constexpr int kStreamBoxBytes = kStreamFeatures * kBlock;
+constexpr int kStreamStageBytes = kStreamWarps * kStreamBoxBytes;
+constexpr int kStreamThreads = (kStreamWarps + 1) * kWarp;
 
-template <typename T, int kNT, int kMT, bool kQuant>
-struct StreamLoads {
-  uint4 w[kMT][2][2];  // [16 features][row g, row g + 8][64-byte half]
-  uint4 x[kNT][kQuant ? 4 : 2];
+template <int kNT>
+struct StreamSmem {
+  static constexpr int kRed = kStreamStages * kStreamStageBytes;
+  static constexpr int kRedRow = kStreamFeatures + 1;
+  static constexpr int kRedBytes = kStreamWarps * kNT * 8 * kRedRow * 4;
+  static constexpr int kBars = kRed + 2 * kRedBytes;
+  static constexpr size_t kBytes = 1024 + kBars + 256;
 };
-
-__device__ __forceinline__ uint4 load_once(const void *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -300,158 +371,194 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t word(const uint4 &v, int i) {
-  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
-template <typename T, int kNT, int kMT, bool kQuant>
-__global__ void __launch_bounds__(kStreamWarps *kWarp)
-    fp8_stream_kernel(const Fp8Params p) {
-  constexpr int kFeatures = 16 * kMT;
-  __shared__ float red[kStreamWarps][kNT * 8][kFeatures + 1];
+template <typename T, int kNT>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
+  using S = StreamSmem<kNT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars);
+  uint64_t *empty = full + kStreamStages;
+  int *abort_flag = reinterpret_cast<int *>(empty + kStreamStages);
   const int warp = threadIdx.x / kWarp;
   const int lane = threadIdx.x % kWarp;
-  const int g = lane / 4, t = lane % 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kFeatures;
-  const float *w_scale = p.b_scales + n0 / kBlock * p.num_kb;
-  const T *x = reinterpret_cast<const T *>(p.a);
+  const int tiles = p.n_tiles;
+  const int steps = (p.num_kb + kStreamWarps - 1) / kStreamWarps;  // stages of a tile
 
-  using Loads = StreamLoads<T, kNT, kMT, kQuant>;
-  auto load = [&](Loads &l, int kb) {
-    const int64_t k0 = static_cast<int64_t>(kb) * kBlock + t * 16;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int64_t k = k0 + half * 64;
-      const bool in = k < p.k;  // k is a multiple of 16: all 16 bytes or none
-#pragma unroll
-      for (int mt = 0; mt < kMT; ++mt) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int64_t n = n0 + mt * 16 + r * 8 + g;
-          l.w[mt][r][half] = in && n < p.n ? load_once(p.b + n * p.k + k) : make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStreamStages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], kStreamWarps);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+
+  if (warp == kStreamWarps) {
+    // A lane for each box of a stage.
+    int stage = 0;
+    uint32_t phase = 0, outstanding = 0, parities = 0;
+    for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
+      for (int step = 0; step < steps; ++step) {
+        if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
+          record_timeout(p.err, abort_flag);
+          break;
+        }
+        const int kb0 = step * kStreamWarps;
+        const int boxes = min(kStreamWarps, p.num_kb - kb0);
+        if (lane == 0) ptx::mbar_expect_tx(&full[stage], boxes * kStreamBoxBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          ptx::tma_load_2d(smem + stage * kStreamStageBytes + lane * kStreamBoxBytes, &tm_b,
+                           &full[stage], (kb0 + lane) * kBlock, tile * kStreamFeatures);
+        }
+        outstanding |= 1u << stage;
+        parities = (parities & ~(1u << stage)) | (phase << stage);
+        if (++stage == kStreamStages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
+    }
+    if (aborted(abort_flag)) {
+      for (int s = 0; s < kStreamStages; ++s) {
+        if (outstanding & (1u << s)) ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
+      }
+    }
+  } else {
+    const int g = lane / 4, t = lane % 4;
+    struct Tokens {
+      uint4 x[kNT][2];
+      float s[kNT][2];
+      float w;
+    };
+    // Tokens' codes and scales of one block of k, a step ahead of their use.
+    auto load = [&](Tokens &l, int tile, int kb) {
+      if (kb >= p.num_kb || tile >= tiles) return;
+      const int64_t k = static_cast<int64_t>(kb) * kBlock + t * 32;
+      l.w = __ldg(p.b_scales +
+                  static_cast<int64_t>(tile * kStreamFeatures / kBlock) * p.num_kb + kb);
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         const int64_t m = nt * 8 + g;
-        const bool ok = in && m < p.m;
-        if constexpr (kQuant) {
-          const uint4 *src = reinterpret_cast<const uint4 *>(x + m * p.k + k);
-          l.x[nt][2 * half] = ok ? __ldg(src) : make_uint4(0, 0, 0, 0);
-          l.x[nt][2 * half + 1] = ok ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
-        } else {
-          l.x[nt][half] = ok ? __ldg(reinterpret_cast<const uint4 *>(p.a + m * p.k + k))
-                             : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // k is a multiple of 16: all 16 bytes or none
+          l.x[nt][h] = m < p.m && k + 16 * h < p.k
+                           ? __ldg(reinterpret_cast<const uint4 *>(p.a + m * p.k + k) + h)
+                           : make_uint4(0, 0, 0, 0);
+          // Scales of the lane's two result columns, tokens 2t and 2t + 1.
+          const int64_t c = nt * 8 + 2 * t + h;
+          l.s[nt][h] = c < p.m ? __ldg(p.a_scales + kb * p.a_pitch + c) : 0.0f;
         }
       }
-    }
-  };
-
-  float acc[kMT][kNT][4] = {};
-  Loads next;
-  if (warp < p.num_kb) load(next, warp);
-  for (int kb = warp; kb < p.num_kb; kb += kStreamWarps) {
-    const Loads cur = next;
-    if (kb + kStreamWarps < p.num_kb) load(next, kb + kStreamWarps);
-    const float ws = w_scale[kb];
+    };
+    ptx::grid_dep_wait();  // codes and scales come from the kernel launched before
+    Tokens next;
+    load(next, blockIdx.x, warp);
+    int stage = 0, parity = 0;
+    uint32_t phase = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
+      float acc[kNT][4] = {};
+      for (int step = 0; step < steps; ++step) {
+        const int kb = step * kStreamWarps + warp;
+        const Tokens cur = next;
+        if (step + 1 < steps) {
+          load(next, tile, kb + kStreamWarps);
+        } else {
+          load(next, tile + gridDim.x, warp);
+        }
+        // After a wait that gave up the rest runs through on what is there.
+        if (!aborted(abort_flag) && !ptx::warp_wait(&full[stage], phase) && lane == 0) {
+          record_timeout(p.err, abort_flag);
+        }
+        if (kb < p.num_kb) {
+          const uint32_t row = ptx::smem_addr(smem + stage * kStreamStageBytes +
+                                              warp * kStreamBoxBytes + g * kBlock);
+          uint4 w[2][2];  // [row g, row g + 8][16-byte half]
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      uint4 xc[2];       // token nt * 8 + g's codes
-      float s0, s1;      // scales of the lane's two result columns, tokens 2t and 2t + 1
-      if constexpr (kQuant) {
-        float f[4][8];
-        unsigned m = 0;
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t chunk = static_cast<uint32_t>((2 * t + h) ^ g) << 4;
+            w[0][h] = ptx::ld_shared_v4(row + chunk);
+            w[1][h] = ptx::ld_shared_v4(row + 8 * kBlock + chunk);
+          }
+          ptx::warp_arrive(&empty[stage]);
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            float d[4] = {};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mma_e4m3(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, cur.x[nt][h].x,
+                       cur.x[nt][h].y);
+              mma_e4m3(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, cur.x[nt][h].z,
+                       cur.x[nt][h].w);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              acc[nt][i] = fmaf(cur.s[nt][i & 1] * cur.w, d[i], acc[nt][i]);
+            }
+          }
+        } else {
+          ptx::warp_arrive(&empty[stage]);
+        }
+        if (++stage == kStreamStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      // Two buffers, so one barrier a tile: a buffer is written again only after
+      // the barrier of the tile in between.
+      float *red = reinterpret_cast<float *>(smem + S::kRed + parity * S::kRedBytes);
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const T *e = reinterpret_cast<const T *>(&cur.x[nt][i]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[i][j] = as_float<T>(e[j]);
-          m = max(m, absmax_bits(f[i]));
+          red[(warp * kNT * 8 + nt * 8 + 2 * t + (i & 1)) * S::kRedRow + g + (i & 2) * 4] =
+              acc[nt][i];
         }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float s = fp8_scale(m);
-        const float inv = __frcp_rn(s);
-        const bool fast = fp8_fast(m, s);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint2 lo = fp8_codes(f[2 * half], s, inv, fast);
-          const uint2 hi = fp8_codes(f[2 * half + 1], s, inv, fast);
-          xc[half] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        }
-        s0 = __shfl_sync(0xffffffffu, s, 8 * t);
-        s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-      } else {
-        xc[0] = cur.x[nt][0];
-        xc[1] = cur.x[nt][1];
-        const int64_t m = nt * 8 + 2 * t;
-        const float *scale = p.a_scales + kb * p.a_pitch + m;
-        s0 = m < p.m ? __ldg(scale) : 0.0f;
-        s1 = m + 1 < p.m ? __ldg(scale + 1) : 0.0f;
       }
-      s0 *= ws;
-      s1 *= ws;
+      ptx::named_bar_sync(1, kStreamWarps * kWarp);
+      for (int i = threadIdx.x; i < kNT * 8 * kStreamFeatures; i += kStreamWarps * kWarp) {
+        const int m = i / kStreamFeatures, f = i % kStreamFeatures;
+        const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
+        float v = 0.0f;
 #pragma unroll
-      for (int mt = 0; mt < kMT; ++mt) {
-        float d[4] = {};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            mma_e4m3(d, word(cur.w[mt][0][half], 2 * j), word(cur.w[mt][1][half], 2 * j),
-                     word(cur.w[mt][0][half], 2 * j + 1), word(cur.w[mt][1][half], 2 * j + 1),
-                     word(xc[half], 2 * j), word(xc[half], 2 * j + 1));
+        for (int w = 0; w < kStreamWarps; ++w) v += red[(w * kNT * 8 + m) * S::kRedRow + f];
+        if (m < p.m && n < p.n) {
+          T *y = static_cast<T *>(p.y) + m * p.n + n;
+          if constexpr (std::is_same_v<T, __half>) {
+            *y = __float2half_rn(v);
+          } else {
+            *y = __float2bfloat16_rn(v);
           }
         }
-        acc[mt][nt][0] = fmaf(s0, d[0], acc[mt][nt][0]);
-        acc[mt][nt][1] = fmaf(s1, d[1], acc[mt][nt][1]);
-        acc[mt][nt][2] = fmaf(s0, d[2], acc[mt][nt][2]);
-        acc[mt][nt][3] = fmaf(s1, d[3], acc[mt][nt][3]);
-      }
-    }
-  }
-#pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        red[warp][nt * 8 + 2 * t + (i & 1)][mt * 16 + g + (i & 2) * 4] = acc[mt][nt][i];
-      }
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kNT * 8 * kFeatures; i += kStreamWarps * kWarp) {
-    const int m = i / kFeatures, f = i % kFeatures;
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kStreamWarps; ++w) v += red[w][m][f];
-    if (m < p.m && n0 + f < p.n) {
-      T *y = static_cast<T *>(p.y) + m * p.n + n0 + f;
-      if constexpr (std::is_same_v<T, __half>) {
-        *y = __float2half_rn(v);
-      } else {
-        *y = __float2bfloat16_rn(v);
       }
     }
   }
 }
 
-constexpr int64_t kFusedRows = 8;    // quantised inside the streaming kernel
-constexpr int64_t kStreamRows = 32;  // streamed at all; tiles above
+constexpr int64_t kStreamRows = 16;  // streamed; tiles above
 
-template <typename T, int kNT, bool kQuant>
-int launch_stream(const Fp8Params &p, cudaStream_t s) {
-  // 32 features a CTA halve the work on the tokens; 16 where that leaves SMs idle.
-  // (Four token tiles leave registers for 16 alone.)
-  const int64_t two = (p.n + 31) / 32;
-  if (kNT <= 2 && two >= sm_count()) {
-    fp8_stream_kernel<T, kNT <= 2 ? kNT : 1, 2, kQuant>
-        <<<static_cast<unsigned>(two), kStreamWarps * kWarp, 0, s>>>(p);
-  } else {
-    fp8_stream_kernel<T, kNT, 1, kQuant>
-        <<<static_cast<unsigned>((p.n + 15) / 16), kStreamWarps * kWarp, 0, s>>>(p);
-  }
+template <typename T, int kNT>
+int launch_stream(Fp8Params p, cudaStream_t s) {
+  using S = StreamSmem<kNT>;
+  p.n_tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
+  p.err = device_error_word();
+  if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
+  CUtensorMap tm_b;
+  if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, kStreamFeatures, true)) return st;
+  if (int st = allow_dynamic_smem<fp8_stream_kernel<T, kNT>>(S::kBytes)) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.n_tiles, sm_count())));
+  cfg.blockDim = dim3(kStreamThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  set_programmatic_dependency(attr[0]);
+  cfg.attrs = attr;
+  cfg.numAttrs = p.after_quantise ? 1 : 0;
+  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_stream_kernel<T, kNT>, tm_b, p));
   return check_launch();
 }
 
@@ -567,6 +674,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   if (warp == C::kEpilogueWarps) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
+      ptx::grid_dep_wait();  // the tokens' codes and scales
       int stage = 0, slot = 0;
       uint32_t phase = 0, outstanding = 0, parities = 0;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
@@ -827,13 +935,14 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  set_programmatic_dependency(attr[1]);
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.after_quantise ? 2 : 1;
   CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16>, tm_a, tm_b, tm_scale,
                                   tm_y, p));
   return check_launch();
@@ -841,9 +950,8 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
 
 template <typename T>
 int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
-  if (p.m <= 8) return launch_stream<T, 1, false>(p, s);
-  if (p.m <= 16) return launch_stream<T, 2, false>(p, s);
-  if (p.m <= kStreamRows) return launch_stream<T, 4, false>(p, s);
+  if (p.m <= 8) return launch_stream<T, 1>(p, s);
+  if (p.m <= kStreamRows) return launch_stream<T, 2>(p, s);
   constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
   // The form with the least time by waves of tiles: a 128-block of k takes about
   // 1300 cycles of a pair's 256 x 256 tile, 780 of a 128 x 128 tile and 700 of a
@@ -907,7 +1015,7 @@ int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
   if (block_rows != 1 && block_rows != CF_FP8_BLOCK_SIZE) return CF_ERR_UNSUPPORTED;
   if (rows == 0 || cols == 0) return CF_OK;
   if (!input || !codes || !scales) return CF_ERR_INVALID_ARGUMENT;
-  if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 37)) {
+  if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 30)) {
     return CF_ERR_INVALID_ARGUMENT;
   }
   return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows, 0,
@@ -933,7 +1041,7 @@ int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, int64_t a_scale
 }
 
 size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k) {
-  if (m <= cfb::kFusedRows || k <= 0) return 0;
+  if (m <= 0 || k <= 0) return 0;
   const int64_t blocks = cfb::fp8_scale_pitch(m) * ((k + cfb::kBlock - 1) / cfb::kBlock);
   return cfb::fp8_code_bytes(m, k) + static_cast<size_t>(blocks) * sizeof(float);
 }
@@ -947,21 +1055,17 @@ int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, 
   if (!cfb::aligned_to(x, 16) || !cfb::aligned_to(w_codes, 16) || !cfb::aligned_to(y, 16)) {
     return CF_ERR_MISALIGNED;
   }
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (m <= cfb::kFusedRows) {
-    const cfb::Fp8Params p = cfb::fp8_params(x, nullptr, 0, w_codes, w_scales, y, m, k, n);
-    return dtype == CF_DTYPE_BF16 ? cfb::launch_stream<__nv_bfloat16, 1, true>(p, s)
-                                  : cfb::launch_stream<__half, 1, true>(p, s);
-  }
   if (workspace == nullptr || workspace_bytes < cf_linear_fp8_workspace_bytes(m, k)) {
     return CF_ERR_WORKSPACE;
   }
   if (!cfb::aligned_to(workspace, 16)) return CF_ERR_MISALIGNED;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   uint8_t *codes = static_cast<uint8_t *>(workspace);
   float *scales = reinterpret_cast<float *>(codes + cfb::fp8_code_bytes(m, k));
   const int64_t pitch = cfb::fp8_scale_pitch(m);
   if (int st = cfb::quantize_fp8_any(x, dtype, codes, scales, m, k, 1, pitch, s)) return st;
-  const cfb::Fp8Params p = cfb::fp8_params(codes, scales, pitch, w_codes, w_scales, y, m, k, n);
+  cfb::Fp8Params p = cfb::fp8_params(codes, scales, pitch, w_codes, w_scales, y, m, k, n);
+  p.after_quantise = true;
   return dtype == CF_DTYPE_BF16 ? cfb::matmul_fp8<__nv_bfloat16>(p, s)
                                 : cfb::matmul_fp8<__half>(p, s);
 }

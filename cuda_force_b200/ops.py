@@ -651,8 +651,7 @@ def linear_fp8(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor) -
 
     ``w_codes [out_features, in_features]`` and ``w_scales`` are
     ``quantize_fp8(weight, block_rows=128)``; ``x`` is float16 or bfloat16 and is
-    quantised in blocks of 1 x 128 on the way (in the same launch for up to eight
-    rows).
+    quantised in blocks of 1 x 128 on the way.
     """
     _check_fp8_operand("w", w_codes, w_scales, FP8_BLOCK_SIZE)
     if x.ndim < 1 or x.shape[-1] != w_codes.shape[1]:

@@ -357,9 +357,9 @@ CF_API int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, int64_t 
                          int64_t k, int64_t n, int dtype, cf_stream_t stream);
 
 /* cf_quantize_fp8 of x [m, k] (dtype f16 or bf16) in blocks of 1 x 128, then
- * cf_matmul_fp8 with the weight w [n, k] (nn.Linear layout). Up to 8 rows are
- * one launch and need no workspace; otherwise the codes and scales of x go to
- * `workspace` (cf_linear_fp8_workspace_bytes, 16-byte aligned). x 16-byte aligned. */
+ * cf_matmul_fp8 with the weight w [n, k] (nn.Linear layout), which may begin while
+ * the first still runs. The codes and scales of x go to `workspace`
+ * (cf_linear_fp8_workspace_bytes, 16-byte aligned). x 16-byte aligned. */
 CF_API size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k);
 CF_API int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, void *y,
                          int64_t m, int64_t k, int64_t n, int dtype, void *workspace,

@@ -133,7 +133,7 @@ def test_fp8_entry_points_refuse():
     lin = lambda m=40, k=64, x=F, ws=F, size=1 << 20: lib.cf_linear_fp8(  # noqa: E731
         x, F, F, F, m, k, 64, F16, ws, size, None)
     need = lib.cf_linear_fp8_workspace_bytes(40, 64)
-    assert need == 40 * 64 + 40 * 4 and lib.cf_linear_fp8_workspace_bytes(8, 64) == 0
+    assert need == 40 * 64 + 40 * 4 and lib.cf_linear_fp8_workspace_bytes(0, 64) == 0
     assert lin(size=need - 1) == _abi.CF_ERR_WORKSPACE
     assert lin(ws=None) == _abi.CF_ERR_WORKSPACE
     assert lin(ws=odd) == _abi.CF_ERR_MISALIGNED and lin(x=odd) == _abi.CF_ERR_MISALIGNED
