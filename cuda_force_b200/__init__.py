@@ -12,6 +12,7 @@ from cuda_force_b200.ops import (
     backend_report,
     dequantize_int8,
     fused_residual_rmsnorm,
+    gated_linear,
     gated_residual_rmsnorm,
     kernel_supports,
     linear_fp8,
@@ -41,6 +42,7 @@ __all__ = [
     "backend_report",
     "dequantize_int8",
     "fused_residual_rmsnorm",
+    "gated_linear",
     "gated_residual_rmsnorm",
     "kernel_supports",
     "linear_fp8",

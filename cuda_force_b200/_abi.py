@@ -25,6 +25,9 @@ CF_DTYPE_F32 = 0
 CF_DTYPE_F16 = 1
 CF_DTYPE_BF16 = 2
 
+CF_ACT_SILU = 0
+CF_ACT_GELU = 1
+
 CF_LAYOUT_REF = 0
 CF_LAYOUT_T = 1
 
@@ -96,6 +99,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _int,
         [_p, _p, _p, _p, _p, _p, _p, _i64, _int, _p, _p, _p, _p, _p, _p, _i64, _i64,
          ctypes.c_float, _int, _p, ctypes.c_size_t, _p],
+    ),
+    "cf_gated_linear": (
+        _int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _p]),
+    "cf_gated_linear_backward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "cf_gated_linear_backward": (
+        _int,
+        [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _p, ctypes.c_size_t,
+         _p],
     ),
     "cf_quantize_fp8": (_int, [_p, _int, _p, _p, _i64, _i64, _int, _p]),
     "cf_matmul_fp8": (_int, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _int, _p]),

@@ -25,7 +25,8 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "libcudaforge_b200.so"
 SHIM = PKG / "_C.so"
 
-CUDA_SOURCES = ["abi.cu", "quant.cu", "lora_gemm.cu", "norm.cu", "block_norm.cu", "fp8_linear.cu"]
+CUDA_SOURCES = ["abi.cu", "quant.cu", "lora_gemm.cu", "norm.cu", "block_norm.cu",
+                "fp8_linear.cu", "gated_linear.cu"]
 HEADERS = ["quant_math.cuh", "cf_common.cuh", "ptx.cuh", "gemm_common.cuh"]
 
 NVCC_FLAGS = [

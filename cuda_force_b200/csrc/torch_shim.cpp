@@ -30,6 +30,7 @@
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -527,6 +528,104 @@ std::vector<at::Tensor> gated_residual_rmsnorm_autograd(
                                      residual_scale, eps);
 }
 
+// ---- gated projections
+
+// A copy where the kernels' 16-byte alignment is not met (a slice of a larger tensor).
+at::Tensor aligned16(const at::Tensor &t) {
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
+// x of any leading dimensions; weights [n, k]. With `save`, also g and u.
+std::vector<at::Tensor> gated_forward(const at::Tensor &x, const at::Tensor &w_gate,
+                                      const at::Tensor &w_up, int64_t activation, bool save) {
+  check_cuda(x, "x");
+  check_contiguous(x, "x");
+  const int dtype = dtype_code(x, "x");
+  TORCH_CHECK(dtype != CF_DTYPE_F32, "gated_linear: x must be bfloat16 or float16");
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  for (const auto &[w, name] : {std::pair<const at::Tensor &, const char *>{w_gate, "w_gate"},
+                                {w_up, "w_up"}}) {
+    check_contiguous(w, name);
+    TORCH_CHECK(w.dim() == 2 && w.sizes() == w_gate.sizes() && w.size(1) == x.size(-1), name,
+                " must be [out_features, ", x.size(-1), "], got ", w.sizes());
+    TORCH_CHECK(w.scalar_type() == x.scalar_type() && w.device() == x.device(), name,
+                " must have x's dtype and device");
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t k = x.size(-1), n = w_gate.size(0), m = k > 0 ? x.numel() / k : 0;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  std::vector<at::Tensor> out{at::empty(shape, x.options())};
+  float *gate = nullptr, *up = nullptr;
+  if (save) {
+    for (int i = 0; i < 2; ++i) {
+      out.push_back(at::empty({m, n}, x.options().dtype(at::kFloat)));
+    }
+    gate = out[1].data_ptr<float>();
+    up = out[2].data_ptr<float>();
+  }
+  const at::Tensor xa = aligned16(x), wg = aligned16(w_gate), wu = aligned16(w_up);
+  check_status(cf_gated_linear(xa.const_data_ptr(), wg.const_data_ptr(), wu.const_data_ptr(),
+                               out[0].data_ptr(), gate, up, m, k, n, static_cast<int>(activation),
+                               dtype, current_stream()),
+               "gated_linear");
+  return out;
+}
+
+at::Tensor gated_linear_cuda(const at::Tensor &x, const at::Tensor &w_gate, const at::Tensor &w_up,
+                             int64_t activation) {
+  return gated_forward(x, w_gate, w_up, activation, false)[0];
+}
+
+struct GatedLinearFunction : torch::autograd::Function<GatedLinearFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x,
+                            const at::Tensor &w_gate, const at::Tensor &w_up, int64_t activation) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    std::vector<at::Tensor> out = gated_forward(x, w_gate, w_up, activation, true);
+    ctx->save_for_backward({x, w_gate, w_up, out[1], out[2]});
+    ctx->saved_data["activation"] = activation;
+    return out[0];
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    check_differentiated_once("gated_linear");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor x = aligned16(saved[0]), wg = aligned16(saved[1]), wu = aligned16(saved[2]);
+    const int dtype = dtype_code(x, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor dy = aligned16(grads[0].contiguous());
+    const int64_t k = x.size(-1), n = wg.size(0), m = x.numel() / std::max<int64_t>(k, 1);
+    at::Tensor out[3];
+    for (int i = 0; i < 3; ++i) {
+      if (!ctx->needs_input_grad(i)) continue;
+      const at::Tensor &like = i == 0 ? x : wg;
+      out[i] = m > 0 && n > 0 ? at::empty_like(like) : at::zeros_like(like);
+    }
+    const size_t ws_bytes = cf_gated_linear_backward_workspace_bytes(m, n);
+    at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+    auto ptr = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check_status(cf_gated_linear_backward(
+                     dy.const_data_ptr(), x.const_data_ptr(), wg.const_data_ptr(),
+                     wu.const_data_ptr(), saved[3].data_ptr<float>(), saved[4].data_ptr<float>(),
+                     ptr(out[0]), ptr(out[1]), ptr(out[2]), m, k, n,
+                     static_cast<int>(ctx->saved_data["activation"].toInt()), dtype, ws.data_ptr(),
+                     ws_bytes, current_stream()),
+                 "gated_linear_backward");
+    return {out[0], out[1], out[2], at::Tensor()};
+  }
+};
+
+at::Tensor gated_linear_autograd(const at::Tensor &x, const at::Tensor &w_gate,
+                                 const at::Tensor &w_up, int64_t activation) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad())) {
+    return GatedLinearFunction::apply(x, w_gate, w_up, activation);
+  }
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return gated_linear_cuda(x, w_gate, w_up, activation);
+}
+
 // ---- 8-bit floating point
 
 std::vector<at::Tensor> quantize_fp8_cuda(const at::Tensor &input, int64_t block_rows) {
@@ -581,11 +680,6 @@ void check_fp8_operand(const at::Tensor &codes, const at::Tensor &scales, const 
 
 const uint8_t *code_ptr(const at::Tensor &t) {
   return static_cast<const uint8_t *>(t.const_data_ptr());
-}
-
-// A copy where the kernels' 16-byte alignment is not met (a slice of a larger tensor).
-at::Tensor aligned16(const at::Tensor &t) {
-  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
 }
 
 at::Tensor matmul_fp8_cuda(const at::Tensor &a_codes, const at::Tensor &a_scales,
@@ -752,6 +846,7 @@ TORCH_LIBRARY(cudaforge, m) {
   m.def(
       "gated_residual_rmsnorm(Tensor x, Tensor residual, Tensor weight, Tensor? post_weight, "
       "Tensor? gate, int gate_groups, float residual_scale, float eps) -> Tensor[]");
+  m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, int activation) -> Tensor");
   m.def("quantize_fp8(Tensor input, int block_rows) -> Tensor[]");
   m.def(
       "matmul_fp8(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, "
@@ -767,6 +862,7 @@ TORCH_LIBRARY_IMPL(cudaforge, Autograd, m) {
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
   }
   m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_autograd);
+  m.impl("gated_linear", &gated_linear_autograd);
 }
 
 TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
@@ -779,6 +875,7 @@ TORCH_LIBRARY_IMPL(cudaforge, CUDA, m) {
   m.impl("rmsnorm", &rmsnorm_cuda);
   m.impl("fused_residual_rmsnorm", &fused_residual_rmsnorm_cuda);
   m.impl("gated_residual_rmsnorm", &gated_residual_rmsnorm_cuda);
+  m.impl("gated_linear", &gated_linear_cuda);
   m.impl("quantize_fp8", &quantize_fp8_cuda);
   m.impl("matmul_fp8", &matmul_fp8_cuda);
   m.impl("linear_fp8", &linear_fp8_cuda);

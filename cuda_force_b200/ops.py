@@ -25,8 +25,8 @@ the reference's names, arguments and messages and take all three dtypes.
 Additive ops: ``lora_linear_int8`` (W as block-INT8 codes + scales),
 ``quantize_dequantize`` (fake quantisation), ``quantize_int8_many`` and, for a
 transformer's feed-forward block, ``gated_residual_rmsnorm``, which is
-differentiable, and the 8-bit floating-point ``quantize_fp8``, ``matmul_fp8``
-and ``linear_fp8``.
+differentiable, as is ``gated_linear``, and the 8-bit floating-point
+``quantize_fp8``, ``matmul_fp8`` and ``linear_fp8``.
 """
 
 from __future__ import annotations
@@ -577,6 +577,53 @@ def lora_linear_int8(
         _as_stored(lora_b), float(scale)
     )
     return y.reshape(*lead, y.shape[-1])
+
+
+#: Activations of :func:`gated_linear`, as the C ABI numbers them.
+GATED_ACTIVATIONS: dict[str, int] = {"silu": 0, "gelu": 1}
+
+
+def gated_linear(
+    x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu"
+) -> torch.Tensor:
+    """``act(x @ w_gate.T) * (x @ w_up.T)``: a feed-forward block's gate and up projections.
+
+    One kernel; the projections, the activation and the product are fp32 and the
+    result is rounded once.
+
+    Args:
+        x: ``[..., in_features]``, float16 or bfloat16.
+        w_gate, w_up: ``[out_features, in_features]`` (nn.Linear layout) in x's dtype.
+        activation: ``"silu"``, or ``"gelu"`` in its tanh form.
+
+    Differentiable in all three, once; the forward pass then keeps both
+    projections in float32. Feature counts that are not multiples of 8 cost
+    zero-padded copies of the operands.
+    """
+    if activation not in GATED_ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, "
+                         f"got {activation!r}")
+    if w_gate.ndim != 2 or w_up.shape != w_gate.shape:
+        raise ValueError("w_gate and w_up must both be [out_features, in_features], got "
+                         f"{tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    n, k = w_gate.shape
+    if x.ndim < 1 or x.shape[-1] != k:
+        raise ValueError(f"x has {x.shape[-1] if x.ndim else 0} input features but the weights "
+                         f"expect {k}")
+    if x.dtype not in INT8_LINEAR_DTYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise ValueError("gated_linear takes float16 or bfloat16 tensors of one dtype, got "
+                         f"{x.dtype}, {w_gate.dtype} and {w_up.dtype}")
+    _require_cuda("gated_linear", x, w_gate, w_up)
+    if k == 0:  # empty sums
+        return (x.new_zeros(*x.shape[:-1], n) + 0 * (w_gate.sum() + w_up.sum() + x.sum()))
+    kp, np_ = -(-k // 8) * 8, -(-n // 8) * 8
+    if kp != k or np_ != n:
+        x = torch.nn.functional.pad(x, (0, kp - k))
+        w_gate = torch.nn.functional.pad(w_gate, (0, kp - k, 0, np_ - n))
+        w_up = torch.nn.functional.pad(w_up, (0, kp - k, 0, np_ - n))
+    y = torch.ops.cudaforge.gated_linear(x.contiguous(), w_gate.contiguous(), w_up.contiguous(),
+                                         GATED_ACTIVATIONS[activation])
+    return y if np_ == n else y[..., :n].contiguous()
 
 
 def _fp8_scale_shape(shape: tuple[int, ...], block_rows: int) -> tuple[int, ...]:

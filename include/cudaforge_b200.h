@@ -329,6 +329,35 @@ CF_API int cf_gated_residual_rmsnorm_backward(
     void *d_post_weight, void *d_gate, int64_t rows, int64_t cols, float residual_scale, int dtype,
     void *workspace, size_t workspace_bytes, cf_stream_t stream);
 
+/* ---- gated projections --------------------------------------------------- */
+
+typedef enum cf_activation {
+  CF_ACT_SILU = 0, /* v / (1 + exp(-v))                                       */
+  CF_ACT_GELU = 1  /* v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2         */
+} cf_activation;
+
+/* y[m, n] = act(g) * u, g = x w_gate^T, u = x w_up^T, x [m, k], weights [n, k]
+ * (nn.Linear layout), all of dtype (f16 or bf16), sums, activation and product in
+ * fp32, y rounded once. gate and up, float [m, n], receive g and u for the
+ * backward pass, or are both NULL. Requirements: k and n multiples of 8, k > 0,
+ * pointers 16-byte aligned. The reference's transformer block runs the two
+ * projections and swiglu apart (examples/transformer_block.py:84-87). */
+CF_API int cf_gated_linear(const void *x, const void *w_gate, const void *w_up, void *y,
+                           float *gate, float *up, int64_t m, int64_t k, int64_t n,
+                           int activation, int dtype, cf_stream_t stream);
+
+/* Gradients of cf_gated_linear for dy [m, n], from its inputs and its gate and up:
+ * dx [m, k], dw_gate and dw_up [n, k], each of dtype and each NULL if not wanted.
+ * dy u act'(g) and dy act(g) are rounded to dtype between the two steps, in
+ * `workspace` (cf_gated_linear_backward_workspace_bytes, 16-byte aligned). Same
+ * requirements. m == 0 or n == 0 writes nothing. */
+CF_API size_t cf_gated_linear_backward_workspace_bytes(int64_t m, int64_t n);
+CF_API int cf_gated_linear_backward(const void *dy, const void *x, const void *w_gate,
+                                    const void *w_up, const float *gate, const float *up,
+                                    void *dx, void *dw_gate, void *dw_up, int64_t m, int64_t k,
+                                    int64_t n, int activation, int dtype, void *workspace,
+                                    size_t workspace_bytes, cf_stream_t stream);
+
 /* ---- 8-bit floating point ------------------------------------------------ */
 
 /* Elements of a row that share a scale, and rows of a weight that do. */

@@ -139,3 +139,51 @@ def test_fp8_entry_points_refuse():
     assert lin(ws=odd) == _abi.CF_ERR_MISALIGNED and lin(x=odd) == _abi.CF_ERR_MISALIGNED
     assert lin(k=24) == _abi.CF_ERR_UNSUPPORTED
     assert lin(m=0) == _abi.CF_OK
+
+
+def test_gated_linear_refuses():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w = torch.zeros(32, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="activation must be one of"):
+        cf.gated_linear(x, w, w, "relu")
+    with pytest.raises(ValueError, match="w_gate and w_up must both be"):
+        cf.gated_linear(x, w, w[:16])
+    with pytest.raises(ValueError, match="input features"):
+        cf.gated_linear(x[:, :32], w, w)
+    with pytest.raises(ValueError, match="one dtype"):
+        cf.gated_linear(x, w, w.half())
+    with pytest.raises(ValueError, match="one dtype"):
+        cf.gated_linear(x.float(), w.float(), w.float())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cf.gated_linear(x, w, w)
+
+
+def test_gated_linear_entry_points_refuse():
+    lib = _abi.load()
+    odd = ctypes.c_void_p(0x1008)
+
+    def fwd(m=4, k=64, n=32, act=0, dt=BF16, x=F, g=None, u=None):
+        return lib.cf_gated_linear(x, F, F, F, g, u, m, k, n, act, dt, None)
+
+    assert fwd(m=-1) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(x=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(act=2) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(g=F) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(m=1 << 31) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(m=1 << 30, n=1 << 30) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert fwd(dt=F32) == _abi.CF_ERR_UNSUPPORTED
+    assert fwd(k=60) == _abi.CF_ERR_UNSUPPORTED and fwd(n=36) == _abi.CF_ERR_UNSUPPORTED
+    assert fwd(k=0) == _abi.CF_ERR_UNSUPPORTED
+    assert fwd(x=odd) == _abi.CF_ERR_MISALIGNED and fwd(g=odd, u=F) == _abi.CF_ERR_MISALIGNED
+    assert fwd(m=0) == _abi.CF_OK and fwd(n=0) == _abi.CF_OK
+    need = lib.cf_gated_linear_backward_workspace_bytes(4, 32)
+    assert need == 512 and lib.cf_gated_linear_backward_workspace_bytes(0, 32) == 0
+
+    def bwd(m=4, g=F, dx=F, ws=F, size=need):
+        return lib.cf_gated_linear_backward(F, F, F, F, g, F, dx, F, F, m, 64, 32, 1, F16, ws, size,
+                                            None)
+
+    assert bwd(g=None) == _abi.CF_ERR_INVALID_ARGUMENT
+    assert bwd(ws=None) == _abi.CF_ERR_WORKSPACE and bwd(size=need - 1) == _abi.CF_ERR_WORKSPACE
+    assert bwd(dx=odd) == _abi.CF_ERR_MISALIGNED and bwd(ws=odd) == _abi.CF_ERR_MISALIGNED
+    assert bwd(m=0) == _abi.CF_OK
