@@ -1,7 +1,7 @@
 // 8-bit floating-point (e4m3) quantisation with a scale for each block of 128,
 // and the matrix product of operands held that way, for sm_100a.
 //
-//   scale = fl32(absmax / 448), 1 when not > 0 (zero, NaN, underflow)
+//   scale = fl32(absmax * fl32(1 / 448)), 1 when not > 0 (zero, NaN, underflow)
 //   code  = e4m3(fl32(x / scale)), nearest even, saturating at +-448, NaN kept
 // over blocks of 1 x 128 (activations) or 128 x 128 (weights); the last block of
 // a row may be shorter. The product of a [m, k] in 1 x 128 blocks and b [n, k]
@@ -24,13 +24,13 @@ namespace cfb {
 namespace {
 
 constexpr int kBlock = CF_FP8_BLOCK_SIZE;
-constexpr float kE4m3Max = 448.0f;
+constexpr float kInvE4m3Max = 1.0f / 448.0f;
 
 // ---------------------------------------------------------------- quantisation
 
 // Scale of a block from the bit pattern of its absmax (a NaN's is the largest).
 __device__ __forceinline__ float fp8_scale(unsigned absmax_bits) {
-  const float s = __fdiv_rn(__uint_as_float(absmax_bits), kE4m3Max);
+  const float s = __fmul_rn(__uint_as_float(absmax_bits), kInvE4m3Max);
   return s > 0.0f ? s : 1.0f;
 }
 

@@ -646,7 +646,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
 
     Blocks are ``block_rows x FP8_BLOCK_SIZE``: 1 row for activations ``[...,
     features]``, ``FP8_BLOCK_SIZE`` rows for a weight ``[out_features,
-    in_features]``. ``scale = absmax / 448`` (1 for a block of zeros) and ``code =
+    in_features]``. ``scale = absmax * (1 / 448)`` in float32 (1 for a block of zeros) and ``code =
     e4m3(x / scale)``, nearest even, saturating. Returns ``(codes, scales)``:
     ``float8_e4m3fn`` shaped like ``x``, and ``[..., ceil(features / 128)]`` or
     ``[ceil(out / 128), ceil(in / 128)]``. The last block of a row or column may

@@ -365,7 +365,7 @@ CF_API int cf_gated_linear_backward(const void *dy, const void *x, const void *w
 
 /* Quantises input [rows, cols] (f32, f16 or bf16, contiguous) to e4m3 codes in
  * blocks of block_rows (1 or CF_FP8_BLOCK_SIZE) x CF_FP8_BLOCK_SIZE elements:
- *   scale = fl32(absmax / 448), replaced by 1 when it is not > 0
+ *   scale = fl32(absmax * fl32(1 / 448)), replaced by 1 when it is not > 0
  *   code  = e4m3(fl32(x / scale)), nearest even, saturating, NaN kept
  * Blocks at the end of a row or column may be smaller. codes: one byte each,
  * [rows, cols]; scales: float [ceil(rows / block_rows)][ceil(cols / 128)]. Any

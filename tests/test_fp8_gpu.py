@@ -1,7 +1,7 @@
 """8-bit floating-point quantisation and products (quantize_fp8, matmul_fp8, linear_fp8).
 
-Codes and scales are defined by single fp32 divisions and one rounding, so they are compared bit
-for bit with torch's. Products are compared with 64-bit products of the dequantised operands: a
+A scale is one fp32 product with the fp32 number next to 1 / 448, a code one fp32 division and one
+rounding, so they are compared bit for bit with torch's. Products are compared with 64-bit products of the dequantised operands: a
 block's 128 products are exact and at most 36 additions deep on the tensor core, each off by at
 most 2^-23 of the block's sum of |products|, and the blocks' sums add 2^-24 each, so with up to
 2^6 blocks the fp32 value is within 2^-17 of the sum of |products|; rounding it adds half a step
@@ -27,7 +27,7 @@ def reference_quantize(x, block_rows):
     wide[:rows, :cols] = x.float()
     blocks = wide.view(rb, block_rows, cb, BLOCK)
     top = blocks.abs().amax((1, 3))
-    scales = top / torch.tensor(448.0, device=x.device)
+    scales = top * (torch.ones((), device=x.device) / torch.full((), 448.0, device=x.device))
     scales = torch.where(scales > 0, scales, torch.ones_like(scales))
     codes = (blocks / scales[:, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
     return codes.view(rb * block_rows, cb * BLOCK)[:rows, :cols].contiguous(), scales
