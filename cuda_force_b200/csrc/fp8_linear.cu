@@ -19,6 +19,7 @@
 #include "cf_common.cuh"
 #include "gemm_common.cuh"
 #include "ptx.cuh"
+#include "stream.cuh"
 
 namespace cfb {
 namespace {
@@ -334,35 +335,13 @@ struct Fp8Params {
   int64_t m, n, k;
   int num_kb;
   int m_tiles, n_tiles, band;
+  int a_rows;  // rows of a in a stage: fewer than a tile's where m ends before
   bool after_quantise;  // a's codes come from the kernel launched just before
   unsigned *err;
 };
 
-// Few rows: bound by reading b once. Persistent CTAs walk over tiles of 16
-// features; a producer warp streams a tile's rows through a 12-stage ring by TMA
-// (192 KB in flight on an SM; registers held too little of it: 24 us at [8, 4096]
-// x [11008, 4096] with loads straight into fragments), 8 blocks of 128 bytes of k
-// a stage, one for each of eight consumer warps. They multiply on the warp-wide
-// MMA (m16n8k32, features as M, tokens as N): at these shapes the tensor core's
-// rate does not matter. A lane's fragment words of a feature are 32 consecutive
-// bytes: within a block any order of k will do as long as both operands use it.
-// The warps' sums of a tile meet in shared memory.
-constexpr int kStreamWarps = 8;
-constexpr int kStreamFeatures = 16;
-constexpr int kStreamStages = 12;
-constexpr int kStreamBoxBytes = kStreamFeatures * kBlock;
-constexpr int kStreamStageBytes = kStreamWarps * kStreamBoxBytes;
-constexpr int kStreamThreads = (kStreamWarps + 1) * kWarp;
-
-template <int kNT>
-struct StreamSmem {
-  static constexpr int kRed = kStreamStages * kStreamStageBytes;
-  static constexpr int kRedRow = kStreamFeatures + 1;
-  static constexpr int kRedBytes = kStreamWarps * kNT * 8 * kRedRow * 4;
-  static constexpr int kBars = kRed + 2 * kRedBytes;
-  static constexpr size_t kBytes = 1024 + kBars + 256;
-};
-
+// Few rows: the streaming kernel with m16n8k32 on e4m3, a box is 16 features of
+// one 128-block of k and a stage eight such blocks.
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 "
@@ -371,195 +350,89 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int kNT>
-__global__ void __launch_bounds__(kStreamThreads, 1)
-    fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_b, const Fp8Params p) {
-  using S = StreamSmem<kNT>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kBars);
-  uint64_t *empty = full + kStreamStages;
-  int *abort_flag = reinterpret_cast<int *>(empty + kStreamStages);
-  const int warp = threadIdx.x / kWarp;
-  const int lane = threadIdx.x % kWarp;
-  const int tiles = p.n_tiles;
-  const int steps = (p.num_kb + kStreamWarps - 1) / kStreamWarps;  // stages of a tile
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStreamStages; ++s) {
-      ptx::mbar_init(&full[s], 1);
-      ptx::mbar_init(&empty[s], kStreamWarps);
-    }
-    *abort_flag = 0;
-    ptx::fence_mbar_init();
-  }
-  __syncthreads();
-
-  if (warp == kStreamWarps) {
-    // A lane for each box of a stage.
-    int stage = 0;
-    uint32_t phase = 0, outstanding = 0, parities = 0;
-    for (int tile = blockIdx.x; tile < tiles && !aborted(abort_flag); tile += gridDim.x) {
-      for (int step = 0; step < steps; ++step) {
-        if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
-          record_timeout(p.err, abort_flag);
-          break;
-        }
-        const int kb0 = step * kStreamWarps;
-        const int boxes = min(kStreamWarps, p.num_kb - kb0);
-        if (lane == 0) ptx::mbar_expect_tx(&full[stage], boxes * kStreamBoxBytes);
-        __syncwarp();
-        if (lane < boxes) {
-          ptx::tma_load_2d(smem + stage * kStreamStageBytes + lane * kStreamBoxBytes, &tm_b,
-                           &full[stage], (kb0 + lane) * kBlock, tile * kStreamFeatures);
-        }
-        outstanding |= 1u << stage;
-        parities = (parities & ~(1u << stage)) | (phase << stage);
-        if (++stage == kStreamStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-    }
-    if (aborted(abort_flag)) {
-      for (int s = 0; s < kStreamStages; ++s) {
-        if (outstanding & (1u << s)) ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
-      }
-    }
-  } else {
-    const int g = lane / 4, t = lane % 4;
-    struct Tokens {
-      uint4 x[kNT][2];
-      float s[kNT][2];
-      float w;
-    };
-    // Tokens' codes and scales of one block of k, a step ahead of their use.
-    auto load = [&](Tokens &l, int tile, int kb) {
-      if (kb >= p.num_kb || tile >= tiles) return;
-      const int64_t k = static_cast<int64_t>(kb) * kBlock + t * 32;
-      l.w = __ldg(p.b_scales +
-                  static_cast<int64_t>(tile * kStreamFeatures / kBlock) * p.num_kb + kb);
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        const int64_t m = nt * 8 + g;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // k is a multiple of 16: all 16 bytes or none
-          l.x[nt][h] = m < p.m && k + 16 * h < p.k
-                           ? __ldg(reinterpret_cast<const uint4 *>(p.a + m * p.k + k) + h)
-                           : make_uint4(0, 0, 0, 0);
-          // Scales of the lane's two result columns, tokens 2t and 2t + 1.
-          const int64_t c = nt * 8 + 2 * t + h;
-          l.s[nt][h] = c < p.m ? __ldg(p.a_scales + kb * p.a_pitch + c) : 0.0f;
-        }
-      }
-    };
-    ptx::grid_dep_wait();  // codes and scales come from the kernel launched before
-    Tokens next;
-    load(next, blockIdx.x, warp);
-    int stage = 0, parity = 0;
-    uint32_t phase = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
-      float acc[kNT][4] = {};
-      for (int step = 0; step < steps; ++step) {
-        const int kb = step * kStreamWarps + warp;
-        const Tokens cur = next;
-        if (step + 1 < steps) {
-          load(next, tile, kb + kStreamWarps);
-        } else {
-          load(next, tile + gridDim.x, warp);
-        }
-        // After a wait that gave up the rest runs through on what is there.
-        if (!aborted(abort_flag) && !ptx::warp_wait(&full[stage], phase) && lane == 0) {
-          record_timeout(p.err, abort_flag);
-        }
-        if (kb < p.num_kb) {
-          const uint32_t row = ptx::smem_addr(smem + stage * kStreamStageBytes +
-                                              warp * kStreamBoxBytes + g * kBlock);
-          uint4 w[2][2];  // [row g, row g + 8][16-byte half]
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t chunk = static_cast<uint32_t>((2 * t + h) ^ g) << 4;
-            w[0][h] = ptx::ld_shared_v4(row + chunk);
-            w[1][h] = ptx::ld_shared_v4(row + 8 * kBlock + chunk);
-          }
-          ptx::warp_arrive(&empty[stage]);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            float d[4] = {};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              mma_e4m3(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, cur.x[nt][h].x,
-                       cur.x[nt][h].y);
-              mma_e4m3(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, cur.x[nt][h].z,
-                       cur.x[nt][h].w);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              acc[nt][i] = fmaf(cur.s[nt][i & 1] * cur.w, d[i], acc[nt][i]);
-            }
-          }
-        } else {
-          ptx::warp_arrive(&empty[stage]);
-        }
-        if (++stage == kStreamStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-      // Two buffers, so one barrier a tile: a buffer is written again only after
-      // the barrier of the tile in between.
-      float *red = reinterpret_cast<float *>(smem + S::kRed + parity * S::kRedBytes);
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          red[(warp * kNT * 8 + nt * 8 + 2 * t + (i & 1)) * S::kRedRow + g + (i & 2) * 4] =
-              acc[nt][i];
-        }
-      }
-      ptx::named_bar_sync(1, kStreamWarps * kWarp);
-      for (int i = threadIdx.x; i < kNT * 8 * kStreamFeatures; i += kStreamWarps * kWarp) {
-        const int m = i / kStreamFeatures, f = i % kStreamFeatures;
-        const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kStreamWarps; ++w) v += red[(w * kNT * 8 + m) * S::kRedRow + f];
-        if (m < p.m && n < p.n) {
-          T *y = static_cast<T *>(p.y) + m * p.n + n;
-          if constexpr (std::is_same_v<T, __half>) {
-            *y = __float2half_rn(v);
-          } else {
-            *y = __float2bfloat16_rn(v);
-          }
-        }
-      }
-    }
-  }
-}
-
-constexpr int64_t kStreamRows = 16;  // streamed; tiles above
-
-template <typename T, int kNT>
-int launch_stream(Fp8Params p, cudaStream_t s) {
-  using S = StreamSmem<kNT>;
-  p.n_tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
-  p.err = device_error_word();
-  if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
+template <typename T>
+struct Fp8StreamOp {
   CUtensorMap tm_b;
-  if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, kStreamFeatures, true)) return st;
-  if (int st = allow_dynamic_smem<fp8_stream_kernel<T, kNT>>(S::kBytes)) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.n_tiles, sm_count())));
-  cfg.blockDim = dim3(kStreamThreads);
-  cfg.dynamicSmemBytes = S::kBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  set_programmatic_dependency(attr[0]);
-  cfg.attrs = attr;
-  cfg.numAttrs = p.after_quantise ? 1 : 0;
-  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_stream_kernel<T, kNT>, tm_b, p));
-  return check_launch();
+  Fp8Params p;
+  unsigned *err;
+  int tiles, steps;
+
+  struct Tokens {
+    uint4 x[2];
+    float s[2];
+    float w;
+  };
+
+  __device__ __forceinline__ void begin() const {
+    ptx::grid_dep_wait();  // codes and scales come from the kernel launched before
+  }
+
+  __device__ __forceinline__ unsigned boxes(int step) const {
+    return (1u << min(kStreamWarps, p.num_kb - step * kStreamWarps)) - 1u;
+  }
+
+  __device__ __forceinline__ void load_box(uint8_t *dst, uint64_t *bar, int tile, int step,
+                                           int box) const {
+    ptx::tma_load_2d(dst, &tm_b, bar, (step * kStreamWarps + box) * kBlock,
+                     tile * kStreamFeatures);
+  }
+
+  __device__ __forceinline__ void load(Tokens &l, int tile, int step, int warp) const {
+    const int kb = step * kStreamWarps + warp;
+    if (kb >= p.num_kb || tile >= tiles) return;
+    const int lane = threadIdx.x % kWarp, g = lane / 4, t = lane % 4;
+    const int64_t k = static_cast<int64_t>(kb) * kBlock + t * 32;
+    l.w = __ldg(p.b_scales + static_cast<int64_t>(tile * kStreamFeatures / kBlock) * p.num_kb + kb);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // k is a multiple of 16: all 16 bytes or none
+      l.x[h] = g < p.m && k + 16 * h < p.k
+                   ? __ldg(reinterpret_cast<const uint4 *>(p.a + g * p.k + k) + h)
+                   : make_uint4(0, 0, 0, 0);
+      // Scales of the lane's two result columns, tokens 2t and 2t + 1.
+      l.s[h] = 2 * t + h < p.m ? __ldg(p.a_scales + kb * p.a_pitch + 2 * t + h) : 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void multiply(const StreamRows &r, const Tokens &l,
+                                           float (&acc)[4]) const {
+    float d[2][4] = {};  // two chains of two
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mma_e4m3(d[h], r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, l.x[h].x, l.x[h].y);
+      mma_e4m3(d[h], r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, l.x[h].z, l.x[h].w);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(l.s[i & 1] * l.w, d[0][i] + d[1][i], acc[i]);
+  }
+
+  __device__ __forceinline__ void store(int tile, const float *red) const {
+    if (threadIdx.x >= kStreamTokens * kStreamFeatures) return;
+    const int m = threadIdx.x / kStreamFeatures, f = threadIdx.x % kStreamFeatures;
+    const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStreamWarps; ++w) v += red[(w * kStreamTokens + m) * kStreamRedRow + f];
+    if (m < p.m && n < p.n) {
+      T *y = static_cast<T *>(p.y) + m * p.n + n;
+      if constexpr (std::is_same_v<T, __half>) {
+        *y = __float2half_rn(v);
+      } else {
+        *y = __float2bfloat16_rn(v);
+      }
+    }
+  }
+};
+
+template <typename T>
+int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
+  Fp8StreamOp<T> op;
+  op.p = p;
+  op.err = device_error_word();
+  if (op.err == nullptr) return record_cuda_error(cudaGetLastError());
+  op.tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
+  op.steps = (p.num_kb + kStreamWarps - 1) / kStreamWarps;
+  if (int st = make_map(&op.tm_b, p.b, 1, p.k, p.n, kBlock, kStreamFeatures, true)) return st;
+  return launch_stream(op, p.after_quantise, s);
 }
 
 // Many rows: tiles on tcgen05, 128 tokens a CTA and kN features. One MMA group
@@ -689,16 +562,17 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
           }
           uint8_t *sa = smem + stage * C::kOperandBytes;
           uint8_t *scale = smem + C::kScaleOffset + slot * C::kScaleBytes;
-          constexpr uint32_t kBytes = C::kOperandBytes + C::kScaleBytes;
+          const uint32_t bytes =
+              C::kOperandBytes + C::kScaleBytes - (kTileM - p.a_rows) * kBlock;
           if constexpr (kCtas == 2) {
             // The even CTA's barrier counts both CTAs' bytes.
             const uint32_t bar = ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0);
-            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * kBytes);
+            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * bytes);
             ptx::tma_load_2d_pair(sa, &tm_a, bar, kb * kBlock, a_row);
             ptx::tma_load_2d_pair(sa + C::kABytes, &tm_b, bar, kb * kBlock, b_row);
             ptx::tma_load_2d_pair(scale, &tm_scale, bar, a_row, kb);
           } else {
-            ptx::mbar_expect_tx(&full[stage], kBytes);
+            ptx::mbar_expect_tx(&full[stage], bytes);
             ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, a_row);
             ptx::tma_load_2d(sa + C::kABytes, &tm_b, &full[stage], kb * kBlock, b_row);
             ptx::tma_load_2d(scale, &tm_scale, &full[stage], a_row, kb);
@@ -918,7 +792,11 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
   CUtensorMap tm_a, tm_b, tm_scale, tm_y;
-  if (int st = make_map(&tm_a, p.a, 1, p.k, p.m, kBlock, kTileM, true)) return st;
+  // A lone tile loads only the rows there are (whole groups of eight, the
+  // swizzle's unit): the others' sums come from what is in shared memory and are
+  // not stored. A full box on a matrix of a few rows loads slowly.
+  p.a_rows = static_cast<int>(std::min<int64_t>(kTileM, (p.m + 7) / 8 * 8));
+  if (int st = make_map(&tm_a, p.a, 1, p.k, p.m, kBlock, p.a_rows, true)) return st;
   if (int st = make_map(&tm_b, p.b, 1, p.k, p.n, kBlock, C::kBRows, true)) return st;
   if (int st = make_map(&tm_scale, p.a_scales, 4, p.m, p.num_kb, kTileM, 1, false, p.a_pitch)) {
     return st;
@@ -950,8 +828,7 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
 
 template <typename T>
 int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
-  if (p.m <= 8) return launch_stream<T, 1>(p, s);
-  if (p.m <= kStreamRows) return launch_stream<T, 2>(p, s);
+  if (p.m <= kStreamTokens) return launch_fp8_stream<T>(p, s);
   constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
   // The form with the least time by waves of tiles: a 128-block of k takes about
   // 1300 cycles of a pair's 256 x 256 tile, 780 of a 128 x 128 tile and 700 of a

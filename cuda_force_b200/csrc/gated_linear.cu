@@ -14,7 +14,8 @@
 // operands' type, which the tensor core's 16-bit products need.
 //
 // Tensor-bound: 4 m n k forward, 8 m n k backward. One tile kernel serves the
-// three products, with K-major or MN-major operands as they lie in memory.
+// three products, with K-major or MN-major operands as they lie in memory. Up to
+// 8 tokens the forward pass is bound by the weights' bytes and streams them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -24,6 +25,7 @@
 #include "cf_common.cuh"
 #include "gemm_common.cuh"
 #include "ptx.cuh"
+#include "stream.cuh"
 
 namespace cfb {
 namespace {
@@ -70,6 +72,7 @@ struct GatedParams {
   int split_kb;    // kInput: blocks of the first of its two products
   int m_tiles, n_tiles, band;
   int matrices;    // kWeights: 1 or 2 gradients
+  int a_rows;      // kForward: rows of x in a stage, fewer than a tile's where m ends before
   int act;
   bool save;       // kForward: keep g and u
   const void *x, *w_gate, *w_up;
@@ -177,7 +180,9 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
           // The even CTA's barrier counts both CTAs' bytes.
           const uint32_t bar = kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0)
                                           : ptx::smem_addr(&full[stage]);
-          if (rank == 0) ptx::mbar_expect_tx(&full[stage], kCtas * C::kStageBytes);
+          const uint32_t bytes =
+              kMode == kForward ? C::kStageBytes - (kTileRows - p.a_rows) * 128 : C::kStageBytes;
+          if (rank == 0) ptx::mbar_expect_tx(&full[stage], kCtas * bytes);
           auto load = [&](uint8_t *dst, const CUtensorMap *map, int c0, int c1) {
             if constexpr (kCtas == 2) {
               ptx::tma_load_2d_pair(dst, map, bar, c0, c1);
@@ -456,6 +461,119 @@ int launch_tiles(const GatedMaps &maps, GatedParams p, int64_t rows, int64_t col
   return check_launch();
 }
 
+// ---------------------------------------------------------------- few tokens
+
+// The streaming kernel with m16n8k16: a box is 16 features of a 64-block of k, a
+// stage four blocks of Wg (warps 0-3) and the same of Wu (warps 4-7).
+constexpr int kStreamBlocks = kStreamWarps / 2;
+
+template <bool kBf16>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+template <bool kBf16>
+struct GatedStreamOp {
+  CUtensorMap tm_w[2];
+  GatedParams p;
+  float *gate, *up;  // g and u for the backward pass, or null
+  unsigned *err;
+  int tiles, steps;
+
+  struct Tokens {
+    uint4 x[2];
+  };
+
+  __device__ __forceinline__ void begin() const {}
+
+  __device__ __forceinline__ unsigned boxes(int step) const {
+    const unsigned half = (1u << min(kStreamBlocks, p.num_kb - step * kStreamBlocks)) - 1u;
+    return half | half << kStreamBlocks;
+  }
+
+  __device__ __forceinline__ void load_box(uint8_t *dst, uint64_t *bar, int tile, int step,
+                                           int box) const {
+    ptx::tma_load_2d(dst, &tm_w[box / kStreamBlocks], bar,
+                     (step * kStreamBlocks + box % kStreamBlocks) * kDepth,
+                     tile * kStreamFeatures);
+  }
+
+  __device__ __forceinline__ void load(Tokens &l, int tile, int step, int warp) const {
+    const int kb = step * kStreamBlocks + warp % kStreamBlocks;
+    if (kb >= p.num_kb || tile >= tiles) return;
+    const int lane = threadIdx.x % kWarp, g = lane / 4, t = lane % 4;
+    const int64_t k = static_cast<int64_t>(kb) * kDepth + t * 16;
+    const uint4 *src =
+        reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.x) + g * p.k + k);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // k is a multiple of 8: all 16 bytes or none
+      l.x[h] = g < p.m && k + 8 * h < p.k ? __ldg(src + h) : make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void multiply(const StreamRows &r, const Tokens &l,
+                                           float (&acc)[4]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mma_16x8x16<kBf16>(acc, r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, l.x[h].x,
+                         l.x[h].y);
+      mma_16x8x16<kBf16>(acc, r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, l.x[h].z,
+                         l.x[h].w);
+    }
+  }
+
+  __device__ __forceinline__ void store(int tile, const float *red) const {
+    if (threadIdx.x >= kStreamTokens * kStreamFeatures) return;
+    const int m = threadIdx.x / kStreamFeatures, f = threadIdx.x % kStreamFeatures;
+    const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
+    float g = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStreamBlocks; ++w) {
+      g += red[(w * kStreamTokens + m) * kStreamRedRow + f];
+      u += red[((w + kStreamBlocks) * kStreamTokens + m) * kStreamRedRow + f];
+    }
+    if (m < p.m && n < p.n) {
+      const int64_t at = m * p.n + n;
+      const float v = g * gate_sigmoid(g, p.act) * u;
+      static_cast<uint16_t *>(p.y)[at] = static_cast<uint16_t>(pack2<kBf16>(v, 0.0f));
+      if (gate != nullptr) {
+        gate[at] = g;
+        up[at] = u;
+      }
+    }
+  }
+};
+
+template <bool kBf16>
+int launch_gated_stream(const GatedParams &p, float *gate, float *up, cudaStream_t s) {
+  GatedStreamOp<kBf16> op;
+  op.p = p;
+  op.gate = gate;
+  op.up = up;
+  op.err = device_error_word();
+  if (op.err == nullptr) return record_cuda_error(cudaGetLastError());
+  op.tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
+  op.steps = (p.num_kb + kStreamBlocks - 1) / kStreamBlocks;
+  const void *w[2] = {p.w_gate, p.w_up};
+  for (int i = 0; i < 2; ++i) {
+    if (int st = make_map(&op.tm_w[i], w[i], 2, p.k, p.n, kDepth, kStreamFeatures, true)) {
+      return st;
+    }
+  }
+  return launch_stream(op, false, s);
+}
+
 // ---------------------------------------------------------------- dg and du
 
 // Elementwise and HBM-bound: reads dy, g and u, writes dg and du (14 bytes an
@@ -489,11 +607,16 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------- host
 
 template <bool kBf16>
-int forward(const GatedParams &p, float *g, float *u, cudaStream_t s) {
+int forward(GatedParams p, float *g, float *u, cudaStream_t s) {
+  if (p.m <= kStreamTokens) return launch_gated_stream<kBf16>(p, g, u, s);
   GatedMaps maps;
   const void *w[2] = {p.w_gate, p.w_up};
   float *save[2] = {g, u};
-  if (int st = make_map(&maps.a[0], p.x, 2, p.k, p.m, kDepth, kTileRows, true)) return st;
+  // A lone tile loads only the rows there are (whole groups of eight, the
+  // swizzle's unit): the others' sums come from what is in shared memory and are
+  // not stored. A full box on a matrix of a few rows loads slowly.
+  p.a_rows = static_cast<int>(std::min<int64_t>(kTileRows, (p.m + 7) / 8 * 8));
+  if (int st = make_map(&maps.a[0], p.x, 2, p.k, p.m, kDepth, p.a_rows, true)) return st;
   maps.a[1] = maps.a[0];
   for (int i = 0; i < 2; ++i) {
     if (int st = make_map(&maps.b[i], w[i], 2, p.k, p.n, kDepth, 128, true)) return st;
