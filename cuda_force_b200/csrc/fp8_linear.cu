@@ -335,6 +335,7 @@ struct Fp8Params {
   int64_t m, n, k;
   int num_kb;
   int m_tiles, n_tiles, band;
+  int splits;  // CTAs that share a tile's blocks of k
   int a_rows;  // rows of a in a stage: fewer than a tile's where m ends before
   bool after_quantise;  // a's codes come from the kernel launched just before
   unsigned *err;
@@ -452,6 +453,7 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
 // that hold them, 32 rows an instruction, cost 0.25 ms). kCtas = 2: CTA pairs,
 // 256 tokens, each CTA staging half of b's rows.
 constexpr int kTileM = 128;
+constexpr int kMaxSplits = 8;  // a portable cluster
 
 template <int kCtas, int kN>
 struct TileCfg {
@@ -485,7 +487,7 @@ struct TileCfg {
   static_assert(kSmem <= 232448, "227 KB of shared memory");
 };
 
-template <int kCtas, int kN, bool kBf16>
+template <int kCtas, int kN, bool kBf16, bool kSplit>
 __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const __grid_constant__ CUtensorMap tm_b,
@@ -504,9 +506,14 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
   const int warp = threadIdx.x / kWarp;
   const int lane = threadIdx.x % kWarp;
+  static_assert(!kSplit || kCtas == 1, "a cluster is a pair or shares a tile's k");
   const uint32_t rank = kCtas == 2 ? ptx::cluster_ctarank() : 0;
   const int tiles = p.m_tiles * p.n_tiles;
-  const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
+  const int share = kSplit ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const int first = blockIdx.x / (kSplit ? p.splits : kCtas);
+  const int step = kSplit ? tiles : gridDim.x / kCtas;
+  const int kb_begin = kSplit ? p.num_kb * share / p.splits : 0;
+  const int kb_end = kSplit ? p.num_kb * (share + 1) / p.splits : p.num_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -555,7 +562,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
         band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
         const int a_row = (tm * kCtas + static_cast<int>(rank)) * kTileM;
         const int b_row = tn * kN + static_cast<int>(rank) * C::kBRows;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
             record_timeout(p.err, abort_flag);
             break;
@@ -607,7 +614,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!ptx::mbar_wait(&tmem_empty[buf], buf_phase ^ 1) ||
               !ptx::mbar_wait(&full[stage], phase)) {
             record_timeout(p.err, abort_flag);
@@ -679,15 +686,17 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
       // scale of one of the next 32 blocks of k.
       const float *b_scale =
           p.b_scales + static_cast<int64_t>(col0 < p.n ? col0 / kBlock : 0) * p.num_kb;
-      float b_next = lane < p.num_kb ? __ldg(b_scale + lane) : 0.0f, b_lane = 0.0f;
+      float b_next = kb_begin + lane < kb_end ? __ldg(b_scale + kb_begin + lane) : 0.0f;
+      float b_lane = 0.0f;
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
       bool ok = true;
-      for (int kb = 0; kb < p.num_kb; ++kb) {
-        if ((kb & 31) == 0) {
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        const int in_chunk = (kb - kb_begin) & 31;
+        if (in_chunk == 0) {
           b_lane = b_next;
-          if (kb + 32 + lane < p.num_kb) b_next = __ldg(b_scale + kb + 32 + lane);
+          if (kb + 32 + lane < kb_end) b_next = __ldg(b_scale + kb + 32 + lane);
         }
         ok = !__any_sync(0xffffffffu, !ptx::mbar_wait(&tmem_full[buf], buf_phase));
         if (!ok) {
@@ -697,7 +706,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
         ptx::tc_fence_after();
         // The scales landed before the MMAs began, which this barrier follows.
         const float scale =
-            ptx::ld_shared_f32(scale_addr) * __shfl_sync(0xffffffffu, b_lane, kb & 31);
+            ptx::ld_shared_f32(scale_addr) * __shfl_sync(0xffffffffu, b_lane, in_chunk);
         scale_addr += C::kScaleBytes;
         if (scale_addr == scale0 + C::kScaleSlots * C::kScaleBytes) scale_addr = scale0;
 #pragma unroll
@@ -727,40 +736,50 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
         }
       }
       if (!ok) break;
-      if (p.n % 8 == 0) {
-        // 32 columns at a time through this warp's buffer (64-byte rows, 16-byte
-        // chunks swizzled as the tensor map expects, which spreads the banks).
-        const uint32_t out = base + C::kOutOffset + warp * C::kOutBytes;
+      if constexpr (kSplit) {
+        // This share of the sums, column by column, over the spent ring.
+        float *part = reinterpret_cast<float *>(smem) + quarter * 32 + lane;
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 32) {
-          if (lane == 0) ptx::bulk_wait_read<0>();
-          __syncwarp();
+        for (int e = 0; e < kCols; ++e) part[(col + e) * kTileM] = acc[e];
+        continue;
+      }
+      // 32 columns at a time through this warp's buffer (64-byte rows, 16-byte
+      // chunks swizzled as the tensor map expects, which spreads the banks).
+      const uint32_t out = base + C::kOutOffset + warp * C::kOutBytes;
+      const bool by_tma = p.n % 8 == 0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
+      for (int c0 = 0; c0 < kCols; c0 += 32) {
+        if (lane == 0) ptx::bulk_wait_read<0>();
+        __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float lo = acc[c0 + c * 8 + 2 * e], hi = acc[c0 + c * 8 + 2 * e + 1];
-              w[e] = kBf16 ? ptx::pack_bf16x2(lo, hi) : ptx::pack_f16x2(lo, hi);
-            }
-            ptx::st_shared_v4(out + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4),
-                              make_uint4(w[0], w[1], w[2], w[3]));
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float lo = acc[c0 + c * 8 + 2 * e], hi = acc[c0 + c * 8 + 2 * e + 1];
+            w[e] = kBf16 ? ptx::pack_bf16x2(lo, hi) : ptx::pack_f16x2(lo, hi);
           }
+          ptx::st_shared_v4(out + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4),
+                            make_uint4(w[0], w[1], w[2], w[3]));
+        }
+        if (by_tma) {
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < p.m && col0 + c0 < p.n) {
             ptx::tma_store_2d_addr(&tm_y, out, col0 + c0, row0);
             ptx::bulk_commit();
           }
-        }
-      } else if (row0 + lane < p.m) {
-        uint16_t *out = static_cast<uint16_t *>(p.y) + (row0 + lane) * p.n + col0;
-#pragma unroll
-        for (int e = 0; e < kCols; ++e) {
-          if (col0 + e < p.n) {
-            out[e] = static_cast<uint16_t>(kBf16 ? ptx::pack_bf16x2(acc[e], 0.0f)
-                                                 : ptx::pack_f16x2(acc[e], 0.0f));
+        } else {
+          // Rows that are not whole 16-byte units: one row an instruction.
+          __syncwarp();
+          const int64_t n = col0 + c0 + lane;
+          const int rows = min(32, static_cast<int>(min(p.m - row0, int64_t{32})));
+          uint16_t *y = static_cast<uint16_t *>(p.y) + row0 * p.n + n;
+          for (int r = 0; r < rows; ++r, y += p.n) {
+            const uint32_t at = out + r * 64 + (((lane >> 3) ^ (r >> 1 & 3)) << 4) + (lane & 7) * 2;
+            if (n < p.n) *y = ptx::ld_shared_u16(at);
           }
+          __syncwarp();
         }
       }
     }
@@ -771,6 +790,50 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   __syncthreads();
   // Neither CTA leaves while the other's MMAs or arrivals may still reach it.
   if constexpr (kCtas == 2) ptx::cluster_sync();
+  if constexpr (kSplit) {
+    // Every CTA adds its part of the columns over the cluster's shares, in rank
+    // order, and stores it; a thread is a row, so its reads are its neighbours'.
+    ptx::cluster_sync();
+    const int row = (first / p.n_tiles) * kTileM + static_cast<int>(threadIdx.x) % kTileM;
+    const int groups = C::kEpilogueWarps * kWarp / kTileM;
+    const int each = kN / (p.splits * groups);  // columns of a thread
+    const int c0 = (share * groups + static_cast<int>(threadIdx.x) / kTileM) * each;
+    if (threadIdx.x < groups * kTileM && row < p.m) {
+      const uint32_t part = ptx::smem_addr(smem) + (threadIdx.x % kTileM) * 4;
+      uint16_t *y = static_cast<uint16_t *>(p.y) + row * p.n;
+      for (int c = c0; c < c0 + each; c += 4) {  // all loads of four columns in flight
+        float v[kMaxSplits][4];
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) {
+          const uint32_t from = ptx::map_shared_rank(
+              part + c * kTileM * 4, static_cast<uint32_t>(r < p.splits ? r : 0));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[r][j] = 0.0f;
+            if (r < p.splits) v[r][j] = ptx::ld_shared_cluster_f32(from + j * kTileM * 4);
+          }
+        }
+        uint32_t w[2];
+#pragma unroll
+        for (int r = 1; r < kMaxSplits; ++r) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[0][j] += v[r][j];
+        }
+        w[0] = kBf16 ? ptx::pack_bf16x2(v[0][0], v[0][1]) : ptx::pack_f16x2(v[0][0], v[0][1]);
+        w[1] = kBf16 ? ptx::pack_bf16x2(v[0][2], v[0][3]) : ptx::pack_f16x2(v[0][2], v[0][3]);
+        const int64_t n = static_cast<int64_t>(first % p.n_tiles) * kN + c;
+        if (p.n % 4 == 0) {
+          if (n < p.n) *reinterpret_cast<uint2 *>(y + n) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (n + j < p.n) y[n + j] = static_cast<uint16_t>(w[j / 2] >> (j % 2 * 16));
+          }
+        }
+      }
+    }
+    ptx::cluster_sync();  // the others may still read this CTA's share
+  }
   if (warp == C::kEpilogueWarps + 1) {
     ptx::tc_fence_after();
     if constexpr (kCtas == 2) {
@@ -781,14 +844,17 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   }
 }
 
-template <int kCtas, int kN, bool kBf16>
-int launch_tiles(Fp8Params p, cudaStream_t s) {
+// splits > 1: that many CTAs, a cluster, share a tile's blocks of k.
+template <int kCtas, int kN, bool kBf16, bool kSplit = false>
+int launch_tiles(Fp8Params p, cudaStream_t s, int splits = 1) {
   using C = TileCfg<kCtas, kN>;
   p.m_tiles = static_cast<int>((p.m + kCtas * kTileM - 1) / (kCtas * kTileM));
   p.n_tiles = static_cast<int>((p.n + kN - 1) / kN);
   // As many row blocks of a in a band as stay in L2 while b streams past.
   const int64_t fit = (int64_t{32} << 20) / (kCtas * kTileM * std::max<int64_t>(p.k, 1));
   p.band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, fit)));
+  if (kSplit) p.band = 1;  // row by row: a cluster finds its tile by a division
+  p.splits = splits;
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
   CUtensorMap tm_a, tm_b, tm_scale, tm_y;
@@ -806,22 +872,23 @@ int launch_tiles(Fp8Params p, cudaStream_t s) {
   } else {
     tm_y = tm_a;
   }
-  if (int st = allow_dynamic_smem<fp8_tile_kernel<kCtas, kN, kBf16>>(C::kSmem)) return st;
+  if (int st = allow_dynamic_smem<fp8_tile_kernel<kCtas, kN, kBf16, kSplit>>(C::kSmem)) return st;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      kSplit ? tiles * splits : std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.x = kSplit ? splits : kCtas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   set_programmatic_dependency(attr[1]);
   cfg.attrs = attr;
   cfg.numAttrs = p.after_quantise ? 2 : 1;
-  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16>, tm_a, tm_b, tm_scale,
+  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, fp8_tile_kernel<kCtas, kN, kBf16, kSplit>, tm_a, tm_b, tm_scale,
                                   tm_y, p));
   return check_launch();
 }
@@ -840,6 +907,12 @@ int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
   };
   const int64_t pair = cost(256, 256, sms / 2, 1300), wide = cost(128, 128, sms, 780),
                 narrow = cost(128, 64, sms, 700);
+  // Few tiles: clusters share a tile's k, eight blocks at least to each CTA ([64,
+  // 11008] x [4096, 11008] 27 -> 20 us; with four [64, 4096] x [1024, 4096] lost 1.6 of 12).
+  const int64_t tiles = (p.m + 127) / 128 * ((p.n + 63) / 64);
+  int splits = 1;
+  while (splits < kMaxSplits && tiles * splits * 2 <= sms && p.num_kb >= splits * 16) splits *= 2;
+  if (splits > 1) return launch_tiles<1, 64, kBf16, true>(p, s, splits);
   if (pair <= wide && pair <= narrow) return launch_tiles<2, 256, kBf16>(p, s);
   return wide <= narrow ? launch_tiles<1, 128, kBf16>(p, s) : launch_tiles<1, 64, kBf16>(p, s);
 }

@@ -711,26 +711,30 @@ at::Tensor matmul_fp8_cuda(const at::Tensor &a_codes, const at::Tensor &a_scales
   return y;
 }
 
-// x [m, k] float16 or bfloat16, quantised on the way; w codes [n, k].
+// x [..., k] float16 or bfloat16, quantised on the way; w codes [n, k].
 at::Tensor linear_fp8_cuda(const at::Tensor &x, const at::Tensor &w_codes,
                            const at::Tensor &w_scales) {
   check_cuda(x, "x");
   check_contiguous(x, "x");
   check_fp8_operand(w_codes, w_scales, "w", CF_FP8_BLOCK_SIZE);
-  TORCH_CHECK(x.dim() == 2, "x must be 2-D, got ", x.dim(), " dimensions");
+  TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
   const int dtype = dtype_code(x, "x");
   TORCH_CHECK(dtype != CF_DTYPE_F32, "linear_fp8: x must be bfloat16 or float16");
   TORCH_CHECK(x.device() == w_codes.device(), "x and w must share a device");
-  const int64_t m = x.size(0), k = x.size(1), n = w_codes.size(0);
+  const int64_t k = x.size(-1), n = w_codes.size(0);
+  int64_t m = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
   TORCH_CHECK(w_codes.size(1) == k, "w codes must be [n, ", k, "], got ", w_codes.sizes());
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor y = at::empty({m, n}, x.options());
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  at::Tensor y = at::empty(shape, x.options());
   if (k == 0) return y.zero_();
   const int64_t kp = (k + 15) / 16 * 16;
   at::Tensor xp = x;
   if (kp != k) {
     xp = at::zeros({m, kp}, x.options());
-    xp.narrow(1, 0, k).copy_(x);
+    xp.narrow(1, 0, k).copy_(x.view({m, k}));
   }
   xp = aligned16(xp);
   const at::Tensor w = aligned16(padded_codes(w_codes, kp));

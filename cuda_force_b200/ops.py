@@ -115,8 +115,10 @@ def _require_cuda(op: str, *tensors: torch.Tensor | None) -> None:
 
 def _require(op: str, *tensors: torch.Tensor) -> None:
     _require_cuda(op, *tensors)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op}: inference-only kernels; no backward is implemented")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{op}: inference-only kernels; no backward is implemented")
 
 
 def _as_stored(t: torch.Tensor) -> torch.Tensor:
@@ -263,18 +265,21 @@ def gated_residual_rmsnorm(
     Differentiable in every tensor, once. Gradients of ``weight``,
     ``post_weight`` and ``gate`` are summed over rows in fp32 in a fixed order.
     """
-    if x.ndim < 1 or x.shape != residual.shape:
+    shape = x.shape
+    if not shape or shape != residual.shape:
         raise ValueError(
-            f"x and residual must have the same shape, got {tuple(x.shape)} "
+            f"x and residual must have the same shape, got {tuple(shape)} "
             f"and {tuple(residual.shape)}"
         )
-    if x.dtype != residual.dtype or x.dtype not in KERNEL_DTYPES:
+    dtype, hidden = x.dtype, shape[-1]
+    if dtype != residual.dtype or dtype not in KERNEL_DTYPES:
         raise ValueError("x and residual must share one dtype of float32, float16 and bfloat16, "
-                         f"got {x.dtype} and {residual.dtype}")
-    hidden = x.shape[-1]
-    for name, w in (("weight", weight), ("post_weight", post_weight)):
-        if w is not None and (w.ndim != 1 or w.shape[0] != hidden):
-            raise ValueError(f"{name} must be 1-D of length {hidden}, got {tuple(w.shape)}")
+                         f"got {dtype} and {residual.dtype}")
+    if weight.shape != (hidden,):
+        raise ValueError(f"weight must be 1-D of length {hidden}, got {tuple(weight.shape)}")
+    if post_weight is not None and post_weight.shape != (hidden,):
+        raise ValueError(f"post_weight must be 1-D of length {hidden}, "
+                         f"got {tuple(post_weight.shape)}")
     groups = 1 if gate is None else _gate_groups(x, gate)
     _require_cuda("gated_residual_rmsnorm", x, residual, weight, post_weight, gate)
     normalised, residual_out = torch.ops.cudaforge.gated_residual_rmsnorm(
@@ -603,14 +608,15 @@ def gated_linear(
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, "
                          f"got {activation!r}")
-    if w_gate.ndim != 2 or w_up.shape != w_gate.shape:
+    shape, dtype = w_gate.shape, x.dtype
+    if len(shape) != 2 or w_up.shape != shape:
         raise ValueError("w_gate and w_up must both be [out_features, in_features], got "
-                         f"{tuple(w_gate.shape)} and {tuple(w_up.shape)}")
-    n, k = w_gate.shape
+                         f"{tuple(shape)} and {tuple(w_up.shape)}")
+    n, k = shape
     if x.ndim < 1 or x.shape[-1] != k:
         raise ValueError(f"x has {x.shape[-1] if x.ndim else 0} input features but the weights "
                          f"expect {k}")
-    if x.dtype not in INT8_LINEAR_DTYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+    if dtype not in INT8_LINEAR_DTYPES or w_gate.dtype != dtype or w_up.dtype != dtype:
         raise ValueError("gated_linear takes float16 or bfloat16 tensors of one dtype, got "
                          f"{x.dtype}, {w_gate.dtype} and {w_up.dtype}")
     _require_cuda("gated_linear", x, w_gate, w_up)
@@ -626,19 +632,19 @@ def gated_linear(
     return y if np_ == n else y[..., :n].contiguous()
 
 
-def _fp8_scale_shape(shape: tuple[int, ...], block_rows: int) -> tuple[int, ...]:
-    return (*shape[:-2], -(-shape[-2] // block_rows), -(-shape[-1] // FP8_BLOCK_SIZE))
-
-
 def _check_fp8_operand(name: str, codes: torch.Tensor, scales: torch.Tensor,
-                       block_rows: int) -> None:
-    if codes.ndim != 2 or codes.dtype != torch.float8_e4m3fn:
+                       block_rows: int) -> int:
+    """The operand's features; its codes and scales have been found to fit."""
+    shape = codes.shape
+    if len(shape) != 2 or codes.dtype != torch.float8_e4m3fn:
         raise ValueError(f"{name}_codes must be a 2-D float8_e4m3fn tensor, got {codes.dtype} "
-                         f"{tuple(codes.shape)}")
-    expected = _fp8_scale_shape(tuple(codes.shape), block_rows)
-    if tuple(scales.shape) != expected or scales.dtype != torch.float32:
+                         f"{tuple(shape)}")
+    rows, features = shape
+    expected = (-(-rows // block_rows), -(-features // FP8_BLOCK_SIZE))
+    if scales.shape != expected or scales.dtype != torch.float32:
         raise ValueError(f"expected float32 block scales {expected} for {name}_codes "
-                         f"{tuple(codes.shape)}, got {scales.dtype} {tuple(scales.shape)}")
+                         f"{tuple(shape)}, got {scales.dtype} {tuple(scales.shape)}")
+    return features
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -681,11 +687,10 @@ def matmul_fp8(
     Products of codes are summed over each block of k and scaled in fp32. ``k``
     that is not a multiple of 16 costs a zero-padded copy of both operands.
     """
-    _check_fp8_operand("a", a_codes, a_scales, 1)
-    _check_fp8_operand("b", b_codes, b_scales, FP8_BLOCK_SIZE)
-    if a_codes.shape[1] != b_codes.shape[1]:
-        raise ValueError(f"a_codes has {a_codes.shape[1]} input features but b_codes expects "
-                         f"{b_codes.shape[1]}")
+    features = _check_fp8_operand("a", a_codes, a_scales, 1)
+    expected = _check_fp8_operand("b", b_codes, b_scales, FP8_BLOCK_SIZE)
+    if features != expected:
+        raise ValueError(f"a_codes has {features} input features but b_codes expects {expected}")
     if dtype not in INT8_LINEAR_DTYPES:
         raise ValueError(f"matmul_fp8 returns float16 or bfloat16, not {dtype}")
     _require("matmul_fp8", a_codes, a_scales, b_codes, b_scales)
@@ -700,15 +705,13 @@ def linear_fp8(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor) -
     ``quantize_fp8(weight, block_rows=128)``; ``x`` is float16 or bfloat16 and is
     quantised in blocks of 1 x 128 on the way.
     """
-    _check_fp8_operand("w", w_codes, w_scales, FP8_BLOCK_SIZE)
-    if x.ndim < 1 or x.shape[-1] != w_codes.shape[1]:
-        raise ValueError(f"x has {x.shape[-1] if x.ndim else 0} input features but weight "
-                         f"expects {w_codes.shape[1]}")
+    features = _check_fp8_operand("w", w_codes, w_scales, FP8_BLOCK_SIZE)
+    shape = x.shape
+    if not shape or shape[-1] != features:
+        raise ValueError(f"x has {shape[-1] if shape else 0} input features but weight "
+                         f"expects {features}")
     if x.dtype not in INT8_LINEAR_DTYPES:
         raise ValueError("linear_fp8 takes float16 or bfloat16 activations")
     _require("linear_fp8", x, w_codes, w_scales)
-    lead = x.shape[:-1]
-    y = torch.ops.cudaforge.linear_fp8(
-        x.reshape(math.prod(lead), x.shape[-1]).contiguous(), w_codes.contiguous(),
-        w_scales.contiguous())
-    return y.view(*lead, y.shape[-1])
+    return torch.ops.cudaforge.linear_fp8(x.contiguous(), w_codes.contiguous(),
+                                          w_scales.contiguous())

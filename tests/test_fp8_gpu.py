@@ -146,6 +146,9 @@ SHAPES = [
     (9, 256, 264), (16, 4096, 4800), (17, 4160, 1030), (32, 1024, 11008), (31, 144, 33),
     (33, 128, 256), (64, 400, 300), (129, 4096, 256), (777, 4160, 1030), (256, 16, 512),
     (1000, 1152, 2051), (4096, 512, 4096), (300, 8192, 384),
+    # few tiles: clusters of 2, 4 and 8 CTAs share a tile's k, ragged shares, odd features
+    (40, 11008, 4096), (20, 1040, 2000), (100, 2064, 1031), (130, 4096, 200), (64, 8192, 64),
+    (9, 4112, 7), (300, 1040, 129),
 ]
 
 
