@@ -444,7 +444,7 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
 //
 // What bounds it is the way from a finished block to a free buffer (barrier,
 // TMEM load, additions, barrier), since TMEM holds two blocks and registers hold
-// 256 features' sums and a quarter of a block. At [16384, 8192] x [28672, 8192]
+// 256 features' sums and an eighth of a block. At [16384, 8192] x [28672, 8192]
 // the MMAs alone take 2.4 ms (3.2 PFLOP/s), the additions 0.6 ms on top. (192
 // features, read at once and the buffer freed before any addition, were no
 // faster.) So everything else is kept off these warps: the tokens' scales come by
@@ -457,15 +457,16 @@ constexpr int kMaxSplits = 8;  // a portable cluster
 
 template <int kCtas, int kN>
 struct TileCfg {
-  static constexpr int kThreadCols = kN >= 128 ? 64 : 32;
-  static constexpr int kEpilogueWarps = 4 * kN / kThreadCols;
+  // Eight epilogue warps: fewer and wider threads have fewer instructions around
+  // the additions (sixteen warps of 64 columns were 4 % slower).
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kThreadCols = kN / 2;
   static constexpr int kThreads = 32 * (kEpilogueWarps + 4);  // + producer, MMA, two idle
-  // Sixteen epilogue warps: 96 registers a thread at launch, moved to where the
-  // sums are (4 * 112 + 32 = 5 * 96), and columns are read 32 at a time. Fewer
-  // warps have registers enough to read their share at once.
-  static constexpr bool kMoveRegs = kEpilogueWarps == 16;
-  static constexpr int kEpilogueRegs = 112, kOtherRegs = 32;
-  static constexpr int kAtOnce = kMoveRegs ? 32 : kThreadCols;
+  // 168 registers a thread at launch; 128 columns' sums need more, which the other
+  // warps give up (2 * 216 + 72 = 3 * 168).
+  static constexpr bool kMoveRegs = kThreadCols == 128;
+  static constexpr int kEpilogueRegs = 216, kOtherRegs = 72;
+  static constexpr int kAtOnce = kMoveRegs ? 32 : kThreadCols;  // columns read at once
   static constexpr int kBRows = kN / kCtas;
   static constexpr int kABytes = kTileM * kBlock;
   static constexpr int kOperandBytes = kABytes + kBRows * kBlock;
@@ -473,7 +474,7 @@ struct TileCfg {
   static constexpr int kOutBytes = 32 * 64;  // a warp's 32 rows x 32 columns on their way out
   static constexpr int kBuffers = 512 / kN < 4 ? 512 / kN : 4;
   static constexpr int kTmemCols = kBuffers * kN <= 256 ? 256 : 512;
-  static constexpr int kStages = kN == 256 ? 5 : 6;
+  static constexpr int kStages = 6;
   // A stage's scales are read by the epilogue, after its operands' slot is free
   // again: the producer's next use of a scale slot has to come after that. It
   // refills operand slot s once the MMAs of kStages blocks ago retired, and those
