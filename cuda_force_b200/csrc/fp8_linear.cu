@@ -98,7 +98,7 @@ struct Eight {
   // `left` of the eight are inside the row, the rest are zeros. kWide: p is on a
   // 16-byte boundary and left is not between 0 and 8.
   template <bool kWide>
-  __device__ __forceinline__ void load(const T *p, int64_t left) {
+  __device__ __forceinline__ void load(const T *p, int left) {
     zero();
     if constexpr (kWide) {
       if (left <= 0) return;
@@ -159,7 +159,7 @@ struct Eight {
 };
 
 template <bool kWide>
-__device__ __forceinline__ void store8(uint8_t *p, int64_t left, uint2 codes) {
+__device__ __forceinline__ void store8(uint8_t *p, int left, uint2 codes) {
   if constexpr (kWide) {
     if (left > 0) *reinterpret_cast<uint2 *>(p) = codes;
   } else {
@@ -172,41 +172,49 @@ __device__ __forceinline__ void store8(uint8_t *p, int64_t left, uint2 codes) {
 }
 
 constexpr int kQuantThreads = 256;
+// Blocks in flight for each half-warp (at [8192, 4096] fp32, two: 29 us, four: 33;
+// at [8192, 11008] bf16, two: 63, four: 58).
+template <typename T>
+constexpr int kQuantUnroll = sizeof(T) == 4 ? 2 : 4;
 
 // 1 x 128 blocks: 16 lanes a block, eight elements a lane; kUnroll blocks a
-// half-warp, loaded before any is reduced.
+// half-warp, loaded before any is reduced. Everything beyond a CTA's first block
+// is 32-bit offsets: at 16 bits an element 64-bit addresses were a third of the
+// instructions, and their registers half of the CTAs that fit on an SM.
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(kQuantThreads)
-    fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks,
-                             int64_t cols, int row_blocks, int64_t scale_row, int64_t scale_kb) {
-  constexpr int kUnroll = 4;
+__global__ void __launch_bounds__(kQuantThreads, 4)
+    fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks, int cols,
+                             int row_blocks, int64_t scale_row, int64_t scale_kb) {
+  constexpr int kUnroll = kQuantUnroll<T>;
   constexpr int kStride = kQuantThreads / 16;
   ptx::grid_dep_launch_dependents();  // a product may fetch its weights meanwhile
   const int lane16 = threadIdx.x & 15;
-  // One division for each CTA; its blocks follow from the first by addition.
-  const int64_t cta_first = static_cast<int64_t>(blockIdx.x) * (kStride * kUnroll);
-  int64_t row = blocks <= 0xffffffffll
-                    ? static_cast<uint32_t>(cta_first) / static_cast<uint32_t>(row_blocks)
-                    : cta_first / row_blocks;
-  int kb = static_cast<int>(cta_first - row * row_blocks) + threadIdx.x / 16;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStride * kUnroll);
+  const int64_t row0 = blocks <= 0xffffffffll
+                           ? static_cast<uint32_t>(first) / static_cast<uint32_t>(row_blocks)
+                           : first / row_blocks;
+  const int here = static_cast<int>(min(blocks - first, int64_t{kStride * kUnroll}));
+  x += row0 * cols;
+  codes += row0 * cols;
+  scales += row0 * scale_row;
+  // (row, kb): this half-warp's block, rows counted from the CTA's first.
+  int row = 0, kb = static_cast<int>(first - row0 * row_blocks) + threadIdx.x / 16;
   Eight<T> v[kUnroll];
-  int64_t at[kUnroll], left[kUnroll], scale_at[kUnroll];
+  int rows[kUnroll], kbs[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     while (kb >= row_blocks) {
       kb -= row_blocks;
       ++row;
     }
+    rows[u] = row;
+    kbs[u] = kb;
     const int c = kb * kBlock + lane16 * 8;
-    at[u] = row * cols + c;
-    scale_at[u] = row * scale_row + kb * scale_kb;
-    left[u] = cta_first + u * kStride + threadIdx.x / 16 < blocks ? cols - c : -1;
-    v[u].template load<kWide>(x + at[u], left[u]);
-    // -1: no such block; 0: a lane behind the end of a row's last block.
-    left[u] = left[u] < -1 ? 0 : left[u];
+    const bool in = static_cast<int>(u * kStride + threadIdx.x / 16) < here;
+    v[u].template load<kWide>(x + (row * cols + c), in ? cols - c : 0);
     kb += kStride;
   }
-  // Each lane divides for one of its half-warp's blocks, not for all of them.
+  // Each lane takes the scale of one of its half-warp's blocks, not of all.
   uint32_t mine = 0;
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
@@ -224,27 +232,34 @@ __global__ void __launch_bounds__(kQuantThreads)
   for (int u = 0; u < kUnroll; ++u) {
     const float s = __shfl_sync(0xffffffffu, my_scale, u, 16);
     const float r = __shfl_sync(0xffffffffu, my_inverse, u, 16);
-    store8<kWide>(codes + at[u], left[u], v[u].codes(s, r, r != 0.0f));
-    if (lane16 == 0 && left[u] > 0) scales[scale_at[u]] = s;
+    const int c = kbs[u] * kBlock + lane16 * 8;
+    const bool in = static_cast<int>(u * kStride + threadIdx.x / 16) < here;
+    store8<kWide>(codes + (rows[u] * cols + c), in ? cols - c : 0,
+                  v[u].codes(s, r, r != 0.0f));
+    if (lane16 == 0 && in) scales[rows[u] * scale_row + kbs[u] * scale_kb] = s;
   }
 }
 
 // 128 x 128 blocks: one CTA each, eight rows of eight elements a thread.
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(kQuantThreads)
-    fp8_quantize_blocks_kernel(const T *x, uint8_t *codes, float *scales, int64_t rows,
-                               int64_t cols) {
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4)
+    fp8_quantize_blocks_kernel(const T *x, uint8_t *codes, float *scales, int64_t rows, int cols) {
   constexpr int kRowsAtOnce = kQuantThreads / 16;
   constexpr int kSteps = kBlock / kRowsAtOnce;
   __shared__ uint32_t warp_top[kQuantThreads / kWarp];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kBlock + (threadIdx.x & 15) * 8;
+  const int c = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
   const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kBlock + threadIdx.x / 16;
+  const int left = cols - c;
+  // Rows of this thread that exist.
+  const int steps = static_cast<int>(
+      min(int64_t{kSteps}, max(int64_t{0}, (rows - r0 + kRowsAtOnce - 1) / kRowsAtOnce)));
+  const int64_t stride = static_cast<int64_t>(kRowsAtOnce) * cols;
   Eight<T> v[kSteps];
   uint32_t top = 0;
+  const T *from = x + r0 * cols + c;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int64_t r = r0 + i * kRowsAtOnce;
-    v[i].template load<kWide>(x + r * cols + c, r < rows ? cols - c : 0);
+  for (int i = 0; i < kSteps; ++i, from += stride) {
+    v[i].template load<kWide>(from, i < steps ? left : 0);
   }
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) top = Eight<T>::larger(top, v[i].top());
@@ -258,12 +273,12 @@ __global__ void __launch_bounds__(kQuantThreads)
   for (int w = 0; w < kQuantThreads / kWarp; ++w) top = Eight<T>::larger(top, warp_top[w]);
   const unsigned m = Eight<T>::bits(top);
   const float s = fp8_scale(m);
-  const float inv = __frcp_rn(s);
   const bool fast = fp8_fast(m, s);
+  const float inv = fast ? __frcp_rn(s) : 0.0f;
+  uint8_t *to = codes + r0 * cols + c;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int64_t r = r0 + i * kRowsAtOnce;
-    store8<kWide>(codes + r * cols + c, r < rows ? cols - c : 0, v[i].codes(s, inv, fast));
+  for (int i = 0; i < kSteps; ++i, to += stride) {
+    store8<kWide>(to, i < steps ? left : 0, v[i].codes(s, inv, fast));
   }
   if (threadIdx.x == 0) scales[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
 }
@@ -276,17 +291,19 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
   const int64_t row_blocks = (cols + kBlock - 1) / kBlock;
   if (block_rows == 1) {
     const int64_t blocks = rows * row_blocks;
-    const int64_t per_cta = kQuantThreads / 16 * 4;
+    const int64_t per_cta = kQuantThreads / 16 * kQuantUnroll<T>;
     const int64_t grid = (blocks + per_cta - 1) / per_cta;
     if (grid > 0x7fffffffll) return CF_ERR_INVALID_ARGUMENT;
     const int64_t scale_row = scale_pitch > 0 ? 1 : row_blocks;
     const int64_t scale_kb = scale_pitch > 0 ? scale_pitch : 1;
     if (wide) {
       fp8_quantize_rows_kernel<T, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, static_cast<int>(row_blocks), scale_row, scale_kb);
+          in, codes, scales, blocks, static_cast<int>(cols), static_cast<int>(row_blocks),
+          scale_row, scale_kb);
     } else {
       fp8_quantize_rows_kernel<T, false><<<static_cast<unsigned>(grid), kQuantThreads, 0, s>>>(
-          in, codes, scales, blocks, cols, static_cast<int>(row_blocks), scale_row, scale_kb);
+          in, codes, scales, blocks, static_cast<int>(cols), static_cast<int>(row_blocks),
+          scale_row, scale_kb);
     }
     return check_launch();
   }
@@ -298,10 +315,12 @@ int quantize_fp8(const void *x, uint8_t *codes, float *scales, int64_t rows, int
     float *to = scales + r / kBlock * row_blocks;
     if (wide) {
       fp8_quantize_blocks_kernel<T, true>
-          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n, cols);
+          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n,
+                                          static_cast<int>(cols));
     } else {
       fp8_quantize_blocks_kernel<T, false>
-          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n, cols);
+          <<<grid, kQuantThreads, 0, s>>>(in + r * cols, codes + r * cols, to, n,
+                                          static_cast<int>(cols));
     }
     if (int st = check_launch()) return st;
   }
