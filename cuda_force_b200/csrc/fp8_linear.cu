@@ -472,8 +472,6 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
 // that hold them, 32 rows an instruction, cost 0.25 ms). kCtas = 2: CTA pairs,
 // 256 tokens, each CTA staging half of b's rows.
 constexpr int kTileM = 128;
-constexpr int kMaxSplits = 8;  // a portable cluster
-
 template <int kCtas, int kN>
 struct TileCfg {
   // Eight epilogue warps: fewer and wider threads have fewer instructions around
@@ -811,48 +809,10 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
   // Neither CTA leaves while the other's MMAs or arrivals may still reach it.
   if constexpr (kCtas == 2) ptx::cluster_sync();
   if constexpr (kSplit) {
-    // Every CTA adds its part of the columns over the cluster's shares, in rank
-    // order, and stores it; a thread is a row, so its reads are its neighbours'.
-    ptx::cluster_sync();
-    const int row = (first / p.n_tiles) * kTileM + static_cast<int>(threadIdx.x) % kTileM;
-    const int groups = C::kEpilogueWarps * kWarp / kTileM;
-    const int each = kN / (p.splits * groups);  // columns of a thread
-    const int c0 = (share * groups + static_cast<int>(threadIdx.x) / kTileM) * each;
-    if (threadIdx.x < groups * kTileM && row < p.m) {
-      const uint32_t part = ptx::smem_addr(smem) + (threadIdx.x % kTileM) * 4;
-      uint16_t *y = static_cast<uint16_t *>(p.y) + row * p.n;
-      for (int c = c0; c < c0 + each; c += 4) {  // all loads of four columns in flight
-        float v[kMaxSplits][4];
-#pragma unroll
-        for (int r = 0; r < kMaxSplits; ++r) {
-          const uint32_t from = ptx::map_shared_rank(
-              part + c * kTileM * 4, static_cast<uint32_t>(r < p.splits ? r : 0));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[r][j] = 0.0f;
-            if (r < p.splits) v[r][j] = ptx::ld_shared_cluster_f32(from + j * kTileM * 4);
-          }
-        }
-        uint32_t w[2];
-#pragma unroll
-        for (int r = 1; r < kMaxSplits; ++r) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[0][j] += v[r][j];
-        }
-        w[0] = kBf16 ? ptx::pack_bf16x2(v[0][0], v[0][1]) : ptx::pack_f16x2(v[0][0], v[0][1]);
-        w[1] = kBf16 ? ptx::pack_bf16x2(v[0][2], v[0][3]) : ptx::pack_f16x2(v[0][2], v[0][3]);
-        const int64_t n = static_cast<int64_t>(first % p.n_tiles) * kN + c;
-        if (p.n % 4 == 0) {
-          if (n < p.n) *reinterpret_cast<uint2 *>(y + n) = make_uint2(w[0], w[1]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n + j < p.n) y[n + j] = static_cast<uint16_t>(w[j / 2] >> (j % 2 * 16));
-          }
-        }
-      }
-    }
-    ptx::cluster_sync();  // the others may still read this CTA's share
+    const int64_t row0 = static_cast<int64_t>(first / p.n_tiles) * kTileM;
+    add_shares<kN, C::kEpilogueWarps * kWarp, kBf16>(
+        ptx::smem_addr(smem), share, p.splits, static_cast<uint16_t *>(p.y) + row0 * p.n, p.n,
+        p.m - row0, static_cast<int64_t>(first % p.n_tiles) * kN, p.n);
   }
   if (warp == C::kEpilogueWarps + 1) {
     ptx::tc_fence_after();
@@ -929,9 +889,7 @@ int matmul_fp8(const Fp8Params &p, cudaStream_t s) {
                 narrow = cost(128, 64, sms, 700);
   // Few tiles: clusters share a tile's k, eight blocks at least to each CTA ([64,
   // 11008] x [4096, 11008] 27 -> 20 us; with four [64, 4096] x [1024, 4096] lost 1.6 of 12).
-  const int64_t tiles = (p.m + 127) / 128 * ((p.n + 63) / 64);
-  int splits = 1;
-  while (splits < kMaxSplits && tiles * splits * 2 <= sms && p.num_kb >= splits * 16) splits *= 2;
+  const int splits = split_count((p.m + 127) / 128 * ((p.n + 63) / 64), p.num_kb, 8);
   if (splits > 1) return launch_tiles<1, 64, kBf16, true>(p, s, splits);
   if (pair <= wide && pair <= narrow) return launch_tiles<2, 256, kBf16>(p, s);
   return wide <= narrow ? launch_tiles<1, 128, kBf16>(p, s) : launch_tiles<1, 64, kBf16>(p, s);

@@ -72,7 +72,8 @@ struct GatedParams {
   int split_kb;    // kInput: blocks of the first of its two products
   int m_tiles, n_tiles, band;
   int matrices;    // kWeights: 1 or 2 gradients
-  int a_rows;      // kForward: rows of x in a stage, fewer than a tile's where m ends before
+  int splits;      // CTAs that share a tile's contracted blocks
+  int a_rows;      // rows of x (or dg, du) in a stage, fewer than a tile's where m ends before
   int act;
   bool save;       // kForward: keep g and u
   const void *x, *w_gate, *w_up;
@@ -111,9 +112,12 @@ struct GatedMaps {
   CUtensorMap a[2], b[2], out[2], save[2];
 };
 
-template <int kMode, int kCtas, bool kBf16>
+// kSplit: the CTAs of a cluster share a tile's contracted blocks and add their
+// sums through distributed shared memory (few tokens leave too few tiles of dx).
+template <int kMode, int kCtas, bool kBf16, bool kSplit>
 __global__ void __launch_bounds__(kGatedThreads, 1)
     gated_tile_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+  static_assert(!kSplit || (kMode == kInput && kCtas == 1), "the split product");
   using C = GatedCfg<kCtas>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
@@ -130,7 +134,11 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   const int rank = kCtas == 2 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   const int per_matrix = p.m_tiles * p.n_tiles;
   const int tiles = per_matrix * (kMode == kWeights ? p.matrices : 1);
-  const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
+  const int share = kSplit ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const int first = blockIdx.x / (kSplit ? p.splits : kCtas);
+  const int step = kSplit ? tiles : gridDim.x / kCtas;
+  const int kb_begin = kSplit ? p.num_kb * share / p.splits : 0;
+  const int kb_end = kSplit ? p.num_kb * (share + 1) / p.splits : p.num_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
         int tm, tn;
         band_order(tile - which * per_matrix, p.m_tiles, p.n_tiles, p.band, tm, tn);
         const int row = (tm * kCtas + rank) * kTileRows;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
             record_timeout(p.err, abort_flag);
             break;
@@ -181,7 +189,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
           const uint32_t bar = kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0)
                                           : ptx::smem_addr(&full[stage]);
           const uint32_t bytes =
-              kMode == kForward ? C::kStageBytes - (kTileRows - p.a_rows) * 128 : C::kStageBytes;
+              kMode == kWeights ? C::kStageBytes : C::kStageBytes - (kTileRows - p.a_rows) * 128;
           if (rank == 0) ptx::mbar_expect_tx(&full[stage], kCtas * bytes);
           auto load = [&](uint8_t *dst, const CUtensorMap *map, int c0, int c1) {
             if constexpr (kCtas == 2) {
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
         bool ok = ptx::mbar_wait(&tmem_empty[buf], buf_phase ^ 1);
         ptx::tc_fence_after();
         const uint32_t d = tmem + buf * kTileCols;
-        for (int kb = 0; ok && kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
           ok = ptx::mbar_wait(&full[stage], phase);
           if (!ok) break;
           ptx::tc_fence_after();
@@ -269,9 +277,9 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < kDepth / 16; ++ks) {
               if constexpr (kCtas == 2) {
-                ptx::mma_f16_pair(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > 0 || ks > 0);
+                ptx::mma_f16_pair(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > kb_begin || ks > 0);
               } else {
-                ptx::mma_f16(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > 0 || ks > 0);
+                ptx::mma_f16(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > kb_begin || ks > 0);
               }
             }
             if constexpr (kCtas == 2) {
@@ -404,6 +412,13 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
           ptx::tmem_ld_32x32b_x32(acc + at, v);
           ptx::tmem_ld_wait();
           if (c == 3) release(buf);
+          if constexpr (kSplit) {
+            // This share of the sums, column by column, over the spent ring.
+            float *part = reinterpret_cast<float *>(smem) + quarter * 32 + lane;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) part[(at + e) * kTileRows] = __uint_as_float(v[e]);
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             w[e] = pack2<kBf16>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
@@ -421,6 +436,12 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   __syncthreads();
   // Neither CTA leaves while the other's MMAs or arrivals may still reach it.
   if constexpr (kCtas == 2) ptx::cluster_sync();
+  if constexpr (kSplit) {
+    const int64_t row0 = static_cast<int64_t>(first / p.n_tiles) * kTileRows;
+    add_shares<kTileCols, 8 * kWarp, kBf16>(
+        ptx::smem_addr(smem), share, p.splits, static_cast<uint16_t *>(p.y) + row0 * p.k, p.k,
+        p.m - row0, static_cast<int64_t>(first % p.n_tiles) * kTileCols, p.k);
+  }
   if (warp == 9) {
     ptx::tc_fence_after();
     if constexpr (kCtas == 2) {
@@ -431,7 +452,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   }
 }
 
-template <int kMode, int kCtas, bool kBf16>
+template <int kMode, int kCtas, bool kBf16, bool kSplit = false>
 int launch_tiles(const GatedMaps &maps, GatedParams p, int64_t rows, int64_t cols, int tile_cols,
                  cudaStream_t s) {
   using C = GatedCfg<kCtas>;
@@ -440,24 +461,26 @@ int launch_tiles(const GatedMaps &maps, GatedParams p, int64_t rows, int64_t col
   // As many row blocks of the A operand in a band as stay in L2 while B streams past.
   const int64_t fit = (int64_t{32} << 20) / (int64_t{kCtas} * kTileRows * p.num_kb * kDepth * 2);
   p.band = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, fit)));
+  if (kSplit) p.band = 1;  // row by row: a cluster finds its tile by a division
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
-  if (int st = allow_dynamic_smem<gated_tile_kernel<kMode, kCtas, kBf16>>(C::kSmem)) return st;
+  if (int st = allow_dynamic_smem<gated_tile_kernel<kMode, kCtas, kBf16, kSplit>>(C::kSmem)) return st;
   const int64_t tiles =
       int64_t{p.m_tiles} * p.n_tiles * (kMode == kWeights ? p.matrices : 1);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      kSplit ? tiles * p.splits : std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas));
   cfg.blockDim = dim3(kGatedThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.x = kSplit ? p.splits : kCtas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, gated_tile_kernel<kMode, kCtas, kBf16>, maps, p));
+  CFB_TRY_CUDA(cudaLaunchKernelEx(&cfg, gated_tile_kernel<kMode, kCtas, kBf16, kSplit>, maps, p));
   return check_launch();
 }
 
@@ -606,16 +629,20 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------- host
 
+// A lone tile loads only the rows there are (whole groups of eight, the swizzle's
+// unit): the others' sums come from what is in shared memory and are not stored. A
+// full box on a matrix of a few rows loads slowly.
+int tile_rows(int64_t m) {
+  return static_cast<int>(std::min<int64_t>(kTileRows, (m + 7) / 8 * 8));
+}
+
 template <bool kBf16>
 int forward(GatedParams p, float *g, float *u, cudaStream_t s) {
   if (p.m <= kStreamTokens) return launch_gated_stream<kBf16>(p, g, u, s);
   GatedMaps maps;
   const void *w[2] = {p.w_gate, p.w_up};
   float *save[2] = {g, u};
-  // A lone tile loads only the rows there are (whole groups of eight, the
-  // swizzle's unit): the others' sums come from what is in shared memory and are
-  // not stored. A full box on a matrix of a few rows loads slowly.
-  p.a_rows = static_cast<int>(std::min<int64_t>(kTileRows, (p.m + 7) / 8 * 8));
+  p.a_rows = tile_rows(p.m);
   if (int st = make_map(&maps.a[0], p.x, 2, p.k, p.m, kDepth, p.a_rows, true)) return st;
   maps.a[1] = maps.a[0];
   for (int i = 0; i < 2; ++i) {
@@ -631,7 +658,7 @@ int forward(GatedParams p, float *g, float *u, cudaStream_t s) {
   // Pairs of CTAs, 256 tokens each, where their tiles keep the GPU as full.
   const int64_t sms = sm_count(), n_tiles = (p.n + 127) / 128;
   const int64_t pairs = (p.m + 255) / 256 * n_tiles, singles = (p.m + 127) / 128 * n_tiles;
-  const bool pair = (pairs + sms / 2 - 1) / (sms / 2) <= (singles + sms - 1) / sms;
+  const bool pair = p.m > kTileRows && (pairs + sms / 2 - 1) / (sms / 2) <= (singles + sms - 1) / sms;
   return pair ? launch_tiles<kForward, 2, kBf16>(maps, p, p.m, p.n, 128, s)
               : launch_tiles<kForward, 1, kBf16>(maps, p, p.m, p.n, 128, s);
 }
@@ -650,14 +677,23 @@ int backward(GatedParams p, const void *dy, const float *g, const float *u, void
   GatedMaps maps;
   if (dx != nullptr) {
     for (int i = 0; i < 2; ++i) {
-      if (int st = make_map(&maps.a[i], d[i], 2, p.n, p.m, kDepth, kTileRows, true)) return st;
+      if (int st = make_map(&maps.a[i], d[i], 2, p.n, p.m, kDepth, tile_rows(p.m), true)) {
+        return st;
+      }
       if (int st = make_map(&maps.b[i], w[i], 2, p.k, p.n, 64, kDepth, true)) return st;
     }
     if (int st = make_map(&maps.out[0], dx, 2, p.k, p.m, 32, 32, true)) return st;
     maps.out[1] = maps.save[0] = maps.save[1] = maps.out[0];
     p.split_kb = static_cast<int>((p.n + kDepth - 1) / kDepth);
     p.num_kb = 2 * p.split_kb;
-    if (int st = launch_tiles<kInput, 2, kBf16>(maps, p, p.m, p.k, kTileCols, s)) return st;
+    p.a_rows = tile_rows(p.m);
+    p.y = dx;
+    p.splits = split_count((p.m + 127) / 128 * ((p.k + kTileCols - 1) / kTileCols), p.num_kb, 16);
+    const int st =
+        p.splits > 1
+            ? launch_tiles<kInput, 1, kBf16, true>(maps, p, p.m, p.k, kTileCols, s)
+            : launch_tiles<kInput, 2, kBf16>(maps, p, p.m, p.k, kTileCols, s);
+    if (st != CF_OK) return st;
   }
   void *dw[2] = {dw_gate, dw_up};
   p.matrices = 0;

@@ -57,6 +57,70 @@ __device__ __forceinline__ void band_order(int t, int rows, int cols, int band, 
   col = i / in_band;
 }
 
+// The end of a product whose contracted dimension a cluster of `splits` CTAs has
+// shared: each left its sums of the 128-row x kCols tile in fp32 at `part`, column
+// by column. Every CTA adds its part of the columns over the shares, in rank
+// order, and stores it as 16-bit numbers into y, the tile's first row, of which
+// `rows` rows and columns [col0, cols) exist. A thread is a row, so its reads are
+// its neighbours'. All threads of the cluster call this.
+constexpr int kMaxSplits = 8;  // a portable cluster
+
+template <int kCols, int kThreads, bool kBf16>
+__device__ __forceinline__ void add_shares(uint32_t part, int share, int splits, uint16_t *y,
+                                           int64_t ldy, int64_t rows, int64_t col0, int64_t cols) {
+  constexpr int kRows = 128;
+  constexpr int kGroups = kThreads / kRows;
+  ptx::cluster_sync();
+  const int row = static_cast<int>(threadIdx.x) % kRows;
+  const int each = kCols / (splits * kGroups);  // columns of a thread
+  const int first = (share * kGroups + static_cast<int>(threadIdx.x) / kRows) * each;
+  if (threadIdx.x < kThreads && row < rows) {
+    y += row * ldy;
+    for (int c = first; c < first + each; c += 4) {  // all loads of four columns in flight
+      float v[kMaxSplits][4];
+#pragma unroll
+      for (int r = 0; r < kMaxSplits; ++r) {
+        const uint32_t from = ptx::map_shared_rank(part + (c * kRows + row) * 4,
+                                                   static_cast<uint32_t>(r < splits ? r : 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[r][j] = 0.0f;
+          if (r < splits) v[r][j] = ptx::ld_shared_cluster_f32(from + j * kRows * 4);
+        }
+      }
+#pragma unroll
+      for (int r = 1; r < kMaxSplits; ++r) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[0][j] += v[r][j];
+      }
+      const uint32_t w[2] = {kBf16 ? ptx::pack_bf16x2(v[0][0], v[0][1])
+                                   : ptx::pack_f16x2(v[0][0], v[0][1]),
+                             kBf16 ? ptx::pack_bf16x2(v[0][2], v[0][3])
+                                   : ptx::pack_f16x2(v[0][2], v[0][3])};
+      const int64_t n = col0 + c;
+      if (ldy % 4 == 0) {
+        if (n < cols) *reinterpret_cast<uint2 *>(y + n) = make_uint2(w[0], w[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j < cols) y[n + j] = static_cast<uint16_t>(w[j / 2] >> (j % 2 * 16));
+        }
+      }
+    }
+  }
+  ptx::cluster_sync();  // the others may still read this CTA's share
+}
+
+// CTAs that share each of `tiles` tiles: as many as the GPU has room for, with
+// `least` blocks at least to each.
+inline int split_count(int64_t tiles, int64_t blocks, int64_t least) {
+  int splits = 1;
+  while (splits < kMaxSplits && tiles * splits * 2 <= sm_count() && blocks >= splits * 2 * least) {
+    splits *= 2;
+  }
+  return splits;
+}
+
 // ---- host: tensor maps and launches
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,

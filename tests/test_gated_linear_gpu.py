@@ -80,6 +80,8 @@ SHAPES = [
     (1, 8, 8), (1, 256, 136), (3, 1000, 520), (8, 4096, 2048), (9, 200, 4000), (16, 72, 24),
     (17, 512, 264), (100, 1024, 1000), (128, 64, 128), (129, 320, 384), (300, 1032, 776),
     (1000, 504, 2056), (2500, 1024, 2048),
+    # few tiles of dx: clusters of 2, 4 and 8 CTAs share its contraction
+    (5, 264, 4104), (130, 1000, 2600), (200, 2048, 1200), (700, 520, 5000),
 ]
 
 
