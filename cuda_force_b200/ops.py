@@ -225,7 +225,7 @@ def _gate_groups(x: torch.Tensor, gate: torch.Tensor) -> int:
         while kept and lead[kept - 1] == 1:
             kept -= 1
         if lead[:kept] == shape[:kept]:
-            return max(1, math.prod(lead))
+            return math.prod(lead)
     raise ValueError(
         f"gate must be [{hidden}], or x's shape with trailing dimensions before the last set "
         f"to 1; got {tuple(gate.shape)} for x {shape}"

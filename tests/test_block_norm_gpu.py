@@ -236,6 +236,11 @@ def test_empty_inputs(cuda_device):
     assert n.shape == h.shape == (0, 64)
     (dw,) = torch.autograd.grad(n.sum() + h.sum(), w)
     assert torch.count_nonzero(dw) == 0 and dw.shape == (64,)
+    gate = torch.zeros(0, 1, 64, device=cuda_device, requires_grad=True)
+    x = torch.zeros(0, 7, 64, device=cuda_device)
+    n, h = cf.gated_residual_rmsnorm(x, x, w, None, gate)
+    (dg,) = torch.autograd.grad(n.sum() + h.sum(), gate)
+    assert n.shape == (0, 7, 64) and dg.shape == gate.shape
 
 
 def test_side_stream_and_graph(cuda_device):
