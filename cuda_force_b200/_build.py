@@ -16,6 +16,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -72,14 +73,17 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
-    objects = []
-    for src in sources:
+
+    def compile_one(src: Path) -> str:
         obj = objdir / (src.stem + ".o")
         cmd = [nvcc, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         _run(cmd)
-        objects.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=min(len(sources), os.cpu_count() or 1)) as pool:
+        objects = list(pool.map(compile_one, sources))
     tmp = LIB.with_suffix(".so.tmp")
     _run([nvcc, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", *objects, "-o", str(tmp)])
     os.replace(tmp, LIB)

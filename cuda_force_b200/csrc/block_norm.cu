@@ -595,8 +595,11 @@ __device__ __forceinline__ void load_staged(const float *w, int c, int cols,
 }
 
 // kShared: a row of the gate serves gate_rows > 1 rows, so its gradient is a
-// sum; otherwise there is none, or one for each row.
-template <typename T, typename TW, int kTpr, bool kShared>
+// sum; otherwise there is none, or one for each row. kFull: the row fills the
+// group's registers exactly, so no chunk is conditional; the branches around them
+// keep the compiler from interleaving the chunks (105 us against 91 at [8192,
+// 4096] bf16).
+template <typename T, typename TW, int kTpr, bool kShared, bool kFull>
 __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
     gated_norm_backward_kernel(const NormArgs a) {
   using S = Wide<T>;
@@ -609,7 +612,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
   const int in_cta = threadIdx.x / kTpr;
   const int t = threadIdx.x % kTpr;
   const int64_t slot = static_cast<int64_t>(blockIdx.x) * kSlots + in_cta;
-  const int cols = static_cast<int>(a.cols);
+  const int cols = kFull ? kTpr * S::kPer : static_cast<int>(a.cols);
   const float inv_cols = 1.0f / static_cast<float>(cols);
   float *post_s = reinterpret_cast<float *>(smem_raw);
   float *weight_s = post_s + cols;
@@ -665,7 +668,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
       for (int i = 0; i < S::kChunks; ++i) {
         const int c = (i * kTpr + t) * S::kVec;
-        if (c < cols) {
+        if (kFull || c < cols) {
           Pair p[kPairs], w[kPairs];
           load_pairs<T, S::kVec>(x + c, p);
           load_pairs<T, S::kVec>(r + c, hh[i]);
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
     for (int i = 0; i < S::kChunks; ++i) {
       const int c = (i * kTpr + t) * S::kVec;
-      if (c < cols) {
+      if (kFull || c < cols) {
         Pair xh[kPairs], w[kPairs], out[kPairs], *d = av[i];
         if (a.dh != nullptr) {
           load_pairs<T, S::kVec>(dh + c, out);
@@ -739,7 +742,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
     for (int i = 0; i < S::kChunks; ++i) {
       const int c = (i * kTpr + t) * S::kVec;
-      if (c < cols) {
+      if (kFull || c < cols) {
         Pair xh[kPairs];
         load_pairs<T, S::kVec>(x + c, xh);
 #pragma unroll
@@ -756,7 +759,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i) {
           const int c = (i * kTpr + t) * S::kVec;
-          if (c < cols) {
+          if (kFull || c < cols) {
             store_pairs<TW, S::kVec>(
                 static_cast<TW *>(a.dgate) + row / a.gate_rows * a.cols + c, sum_g[i]);
           }
@@ -772,7 +775,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
   for (int i = 0; i < S::kChunks; ++i) {
     const int c = (i * kTpr + t) * S::kVec;
-    if (c < cols) {
+    if (kFull || c < cols) {
       store_pairs<float, S::kVec>(part + c, sum_w[i]);
       if (a.post) store_pairs<float, S::kVec>(part + plane + c, sum_p[i]);
       if (kShared && !a.whole_groups) store_pairs<float, S::kVec>(part + 2 * plane + c, sum_g[i]);
@@ -1058,7 +1061,7 @@ __global__ void __launch_bounds__(kFinishCols *kFinishRows)
 
 // Threads for a row of `cols` elements at `per` elements a thread; 0: long row.
 int threads_per_row(int64_t cols, int per) {
-  for (int tpr : {32, 128, 256, 512, 1024}) {
+  for (int tpr : {32, 64, 128, 256, 512, 1024}) {
     if (cols <= static_cast<int64_t>(tpr) * per) return tpr;
   }
   return 0;
@@ -1137,6 +1140,7 @@ template <typename T, typename TW>
 int forward(const NormArgs &a, bool wide, cudaStream_t s) {
   switch (threads_per_row(a.cols, wide ? Wide<T>::kPer : Simple::kPer)) {
     case 32: return launch_forward<T, TW, 32>(a, wide, s);
+    case 64: return launch_forward<T, TW, 64>(a, wide, s);
     case 128: return launch_forward<T, TW, 128>(a, wide, s);
     case 256: return launch_forward<T, TW, 256>(a, wide, s);
     case 512: return launch_forward<T, TW, 512>(a, wide, s);
@@ -1147,6 +1151,11 @@ int forward(const NormArgs &a, bool wide, cudaStream_t s) {
       return check_launch();
   }
 }
+
+template <bool kShared, bool kFull>
+struct BackwardForm {
+  static constexpr bool shared = kShared, full = kFull;
+};
 
 template <typename T, typename TW, int kTpr>
 int launch_backward(const NormArgs &a, bool wide, cudaStream_t s) {
@@ -1166,10 +1175,14 @@ int launch_backward(const NormArgs &a, bool wide, cudaStream_t s) {
   constexpr int kWideTpr =
       std::min<int>(kTpr, static_cast<int>(kBackwardMaxCols / Wide<T>::kPer));
   constexpr int ctas = backward_ctas<kWideTpr>();
-  return shared ? launch_staged<gated_norm_backward_kernel<T, TW, kWideTpr, true>>(
-                      a, 4, sizeof(T), kSlots, grid, kThreads, ctas, s)
-                : launch_staged<gated_norm_backward_kernel<T, TW, kWideTpr, false>>(
-                      a, 4, sizeof(T), kSlots, grid, kThreads, ctas, s);
+  auto run = [&](auto tag) {
+    return launch_staged<gated_norm_backward_kernel<T, TW, kWideTpr, decltype(tag)::shared,
+                                                    decltype(tag)::full>>(
+        a, 4, sizeof(T), kSlots, grid, kThreads, ctas, s);
+  };
+  const bool full = a.cols == kWideTpr * Wide<T>::kPer;
+  if (shared) return full ? run(BackwardForm<true, true>{}) : run(BackwardForm<true, false>{});
+  return full ? run(BackwardForm<false, true>{}) : run(BackwardForm<false, false>{});
 }
 
 template <typename T, typename TW>
@@ -1183,6 +1196,7 @@ int backward(const NormArgs &a, bool wide, void *dweight, void *dpost, cudaStrea
     st = launch_backward<T, TW, tpr>(a, wide, s);  \
     break
     CFB_CASE(32);
+    CFB_CASE(64);
     CFB_CASE(128);
     CFB_CASE(256);
     CFB_CASE(512);
