@@ -233,10 +233,11 @@ constexpr int cta_threads() { return kTpr == kWarp ? kThreadsSmall : kTpr; }
 
 // ---------------------------------------------------------------- forward
 
-// One row for each group of threads, in registers through both passes. The
-// hardware hides one row's two sums behind other CTAs' rows: 58 us at [8192,
-// 4096] bf16 with scalar arithmetic, against 73 us for persistent CTAs with the
-// backward kernel's ring and staged weights.
+// One row for each group of threads, in registers through both passes. What
+// hides a row's two sums is other CTAs' rows, so registers are what bounds it:
+// inputs stay packed, and 1536 threads fit on an SM. [16384, 4096] bf16 with a
+// gate: 87 us, 6.2 TB/s (1024 threads 97 us; unpacked scalar arithmetic 108 us;
+// persistent CTAs with the backward kernel's ring 122 us).
 template <typename T, typename TW, int kTpr>
 __global__ void __launch_bounds__(cta_threads<kTpr>(), 1536 / cta_threads<kTpr>())
     gated_norm_kernel(const NormArgs a) {
@@ -597,8 +598,10 @@ __device__ __forceinline__ void load_staged(const float *w, int c, int cols,
 // kShared: a row of the gate serves gate_rows > 1 rows, so its gradient is a
 // sum; otherwise there is none, or one for each row. kFull: the row fills the
 // group's registers exactly, so no chunk is conditional; the branches around them
-// keep the compiler from interleaving the chunks (105 us against 91 at [8192,
-// 4096] bf16).
+// keep the compiler from interleaving the chunks. [8192, 4096] bf16 with a gate:
+// 91 us (105 with the branches, 157 without the ring), 4.4 TB/s, and 8 us to add
+// the partial sums; bound by instruction issue and latency at the 512 threads an
+// SM has registers for.
 template <typename T, typename TW, int kTpr, bool kShared, bool kFull>
 __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
     gated_norm_backward_kernel(const NormArgs a) {
@@ -1071,12 +1074,12 @@ int threads_per_row(int64_t cols, int per) {
 // The longest row of the staged and simple backward kernels.
 constexpr int64_t kBackwardMaxCols = 8192;
 
-// The backward pass's slots: as many rows at a time as keep the memory busy (512
-// threads an SM; eight rows of a warp each), since more only add partial sums.
+// The backward pass's slots: as many rows at a time as an SM holds (512 threads of
+// them), since more only add partial sums.
 void plan_slots(NormArgs &a, int dtype, bool shared_gate) {
   const int tpr =
       a.cols > kBackwardMaxCols ? 0 : threads_per_row(a.cols, dtype == CF_DTYPE_F32 ? 8 : 16);
-  const int64_t per_sm = tpr == 0 ? 2 : tpr == kWarp ? 8 : std::max(1, 512 / tpr);
+  const int64_t per_sm = tpr == 0 ? 2 : std::max(1, 512 / tpr);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.rows, per_sm * sm_count()));
   const int64_t group_rows = shared_gate ? a.gate_rows : a.rows;
   const int64_t groups = a.rows / group_rows;
@@ -1118,7 +1121,8 @@ int launch_staged(NormArgs a, int arrays, int64_t elem, int groups, unsigned gri
   if (a.stages < 1) return CF_ERR_UNSUPPORTED;  // not for any length the kernels are built for
   a.err = device_error_word();
   if (a.err == nullptr) return record_cuda_error(cudaGetLastError());
-  const size_t smem = 2 * a.cols * 4 + static_cast<size_t>(a.stages) * arrays * a.cols * elem * groups;
+  const size_t smem =
+      2 * a.cols * 4 + static_cast<size_t>(a.stages) * arrays * a.cols * elem * groups;
   if (int st = allow_dynamic_smem<Kernel>(kRingSmem)) return st;
   Kernel<<<grid, threads, smem, s>>>(a);
   return check_launch();
@@ -1223,8 +1227,8 @@ int backward(const NormArgs &a, bool wide, void *dweight, void *dpost, cudaStrea
 }
 
 template <bool kForward>
-int dispatch_norm(const NormArgs &a, int dtype, int weight_dtype, bool wide, void *dweight, void *dpost,
-             cudaStream_t s) {
+int dispatch_norm(const NormArgs &a, int dtype, int weight_dtype, bool wide, void *dweight,
+                  void *dpost, cudaStream_t s) {
   const bool wf = weight_dtype == CF_DTYPE_F32;
 #define CFB_RUN(T, TW)                                       \
   do {                                                       \

