@@ -31,6 +31,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -479,6 +480,14 @@ void check_differentiated_once(const char *op) {
               ": gradients of gradients are not implemented (create_graph=True)");
 }
 
+// Nor do they have tangents, which would be lost without a word.
+void check_no_tangents(const char *op, std::initializer_list<at::Tensor> inputs) {
+  for (const at::Tensor &t : inputs) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), op,
+                ": forward-mode differentiation is not implemented");
+  }
+}
+
 struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
   static torch::autograd::variable_list forward(
       torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &residual,
@@ -517,6 +526,9 @@ std::vector<at::Tensor> gated_residual_rmsnorm_autograd(
     const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight,
     const std::optional<at::Tensor> &post_weight, const std::optional<at::Tensor> &gate,
     int64_t gate_groups, double residual_scale, double eps) {
+  const at::Tensor none;
+  check_no_tangents("gated_residual_rmsnorm", {x, residual, weight, post_weight.value_or(none),
+                                               gate.value_or(none)});
   auto wants = [](const std::optional<at::Tensor> &t) { return t && t->requires_grad(); };
   if (at::GradMode::is_enabled() && (x.requires_grad() || residual.requires_grad() ||
                                      weight.requires_grad() || wants(post_weight) || wants(gate))) {
@@ -618,6 +630,7 @@ struct GatedLinearFunction : torch::autograd::Function<GatedLinearFunction> {
 
 at::Tensor gated_linear_autograd(const at::Tensor &x, const at::Tensor &w_gate,
                                  const at::Tensor &w_up, int64_t activation) {
+  check_no_tangents("gated_linear", {x, w_gate, w_up});
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad())) {
     return GatedLinearFunction::apply(x, w_gate, w_up, activation);

@@ -280,6 +280,9 @@ def gated_residual_rmsnorm(
     if post_weight is not None and post_weight.shape != (hidden,):
         raise ValueError(f"post_weight must be 1-D of length {hidden}, "
                          f"got {tuple(post_weight.shape)}")
+    if isinstance(residual_scale, torch.Tensor):  # it would lose its gradient
+        raise ValueError("residual_scale must be a number; a learnable one can be folded into "
+                         "residual")
     groups = 1 if gate is None else _gate_groups(x, gate)
     _require_cuda("gated_residual_rmsnorm", x, residual, weight, post_weight, gate)
     normalised, residual_out = torch.ops.cudaforge.gated_residual_rmsnorm(

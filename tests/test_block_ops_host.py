@@ -28,6 +28,8 @@ def test_gated_residual_rmsnorm_refuses():
         call(x, x, torch.ones(9))
     with pytest.raises(ValueError, match="post_weight must be 1-D of length 8"):
         call(x, x, w, torch.ones(1, 8))
+    with pytest.raises(ValueError, match="residual_scale must be a number"):
+        call(x, x, w, residual_scale=torch.ones((), requires_grad=True))
     for bad in ((9,), (1, 3, 8), (3, 8), (2, 1, 1), (2, 2, 8)):
         with pytest.raises(ValueError, match="gate must be"):
             call(x, x, w, None, torch.ones(bad))

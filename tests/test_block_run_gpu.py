@@ -117,3 +117,19 @@ def test_two_streams_at_once(cuda_device):
     for want, r in zip(alone, results):
         for got in r:
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_forward_mode_differentiation_is_refused(cuda_device):
+    x = torch.randn(4, 64, device=cuda_device, dtype=torch.bfloat16)
+    w = torch.ones(64, device=cuda_device, dtype=torch.bfloat16)
+    square = torch.zeros(32, 64, device=cuda_device, dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        dual_w = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: cf.gated_residual_rmsnorm(x, dual, w),
+                     lambda: cf.gated_residual_rmsnorm(x, x, w, None, dual_w),
+                     lambda: cf.gated_linear(dual, square, square)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        n, _ = cf.gated_residual_rmsnorm(x, x, w)  # without a tangent nothing changes
+    assert torch.equal(n, cf.gated_residual_rmsnorm(x, x, w)[0])
