@@ -376,67 +376,63 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 
 template <typename T>
 struct Fp8StreamOp {
-  CUtensorMap tm_b;
-  Fp8Params p;
-  unsigned *err;
-  int tiles, steps;
-
-  struct Tokens {
-    uint4 x[2];
-    float s[2];
-    float w;
+  static constexpr int kMatrices = 1, kBlocks = kStreamWarps, kBlockElems = kBlock;
+  static constexpr int kScaleBytes = kStreamWarps * kStreamTokens * 4;
+  // Of the block of the tile's first feature and of the next: a lane holds one of the
+  // next 32 steps.
+  struct Weights {
+    float w[2];
   };
 
-  __device__ __forceinline__ void begin() const {
-    ptx::grid_dep_wait();  // codes and scales come from the kernel launched before
+  StreamMap w[1], less[1], tokens;
+  CUtensorMap tm_scale;
+  Fp8Params p;
+  unsigned *err;
+  StreamTiles tiles;
+  int steps, blocks, token_rows, scale_bytes;
+  bool whole;
+
+  __device__ __forceinline__ void load_scales(uint8_t *dst, uint64_t *bar, int step) const {
+    ptx::tma_load_2d(dst, &tm_scale, bar, 0, step * kStreamWarps);
   }
 
-  __device__ __forceinline__ unsigned boxes(int step) const {
-    return (1u << min(kStreamWarps, p.num_kb - step * kStreamWarps)) - 1u;
-  }
-
-  __device__ __forceinline__ void load_box(uint8_t *dst, uint64_t *bar, int tile, int step,
-                                           int box) const {
-    ptx::tma_load_2d(dst, &tm_b, bar, (step * kStreamWarps + box) * kBlock,
-                     tile * kStreamFeatures);
-  }
-
-  __device__ __forceinline__ void load(Tokens &l, int tile, int step, int warp) const {
-    const int kb = step * kStreamWarps + warp;
-    if (kb >= p.num_kb || tile >= tiles) return;
-    const int lane = threadIdx.x % kWarp, g = lane / 4, t = lane % 4;
-    const int64_t k = static_cast<int64_t>(kb) * kBlock + t * 32;
-    l.w = __ldg(p.b_scales + static_cast<int64_t>(tile * kStreamFeatures / kBlock) * p.num_kb + kb);
+  __device__ __forceinline__ void fetch(Weights &l, int feature, int step, int warp) const {
+    const int64_t kb = int64_t{step + static_cast<int>(threadIdx.x % kWarp)} * kStreamWarps + warp;
+    const int last_block = static_cast<int>((p.n - 1) / kBlock);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // k is a multiple of 16: all 16 bytes or none
-      l.x[h] = g < p.m && k + 16 * h < p.k
-                   ? __ldg(reinterpret_cast<const uint4 *>(p.a + g * p.k + k) + h)
-                   : make_uint4(0, 0, 0, 0);
-      // Scales of the lane's two result columns, tokens 2t and 2t + 1.
-      l.s[h] = 2 * t + h < p.m ? __ldg(p.a_scales + kb * p.a_pitch + 2 * t + h) : 0.0f;
+    for (int h = 0; h < 2; ++h) {
+      const int block = min(feature / kBlock + h, last_block);
+      if (kb < p.num_kb) l.w[h] = __ldg(p.b_scales + int64_t{block} * p.num_kb + kb);
     }
   }
 
-  __device__ __forceinline__ void multiply(const StreamRows &r, const Tokens &l,
-                                           float (&acc)[4]) const {
+  __device__ __forceinline__ void multiply(const StreamRows &r, const uint4 (&x)[2],
+                                           const float (&s)[2], const Weights &l, int feature,
+                                           int step, float (&acc)[4]) const {
     float d[2][4] = {};  // two chains of two
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      mma_e4m3(d[h], r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, l.x[h].x, l.x[h].y);
-      mma_e4m3(d[h], r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, l.x[h].z, l.x[h].w);
+      mma_e4m3(d[h], r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, x[h].x, x[h].y);
+      mma_e4m3(d[h], r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, x[h].z, x[h].w);
     }
+    const float first = __shfl_sync(0xffffffffu, l.w[0], step % kWarp);
+    const float second = __shfl_sync(0xffffffffu, l.w[1], step % kWarp);
+    const int in_block = feature % kBlock + static_cast<int>(threadIdx.x % kWarp) / 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(l.s[i & 1] * l.w, d[0][i] + d[1][i], acc[i]);
+    for (int i = 0; i < 4; ++i) {  // the lane's features, rows g and g + 8
+      const float w = in_block + i / 2 * 8 < kBlock ? first : second;
+      acc[i] = fmaf(s[i & 1] * w, d[0][i] + d[1][i], acc[i]);
+    }
   }
 
-  __device__ __forceinline__ void store(int tile, const float *red) const {
+  __device__ __forceinline__ void store(int feature, int count, const float *red) const {
     if (threadIdx.x >= kStreamTokens * kStreamFeatures) return;
     const int m = threadIdx.x / kStreamFeatures, f = threadIdx.x % kStreamFeatures;
-    const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
+    const int64_t n = int64_t{feature} + f;
     float v = 0.0f;
 #pragma unroll
     for (int w = 0; w < kStreamWarps; ++w) v += red[(w * kStreamTokens + m) * kStreamRedRow + f];
-    if (m < p.m && n < p.n) {
+    if (m < p.m && f < count && n < p.n) {
       T *y = static_cast<T *>(p.y) + m * p.n + n;
       if constexpr (std::is_same_v<T, __half>) {
         *y = __float2half_rn(v);
@@ -453,9 +449,23 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
   op.p = p;
   op.err = device_error_word();
   if (op.err == nullptr) return record_cuda_error(cudaGetLastError());
-  op.tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
+  op.tiles = stream_tiles(p.n);
+  op.blocks = p.num_kb;
   op.steps = (p.num_kb + kStreamWarps - 1) / kStreamWarps;
-  if (int st = make_map(&op.tm_b, p.b, 1, p.k, p.n, kBlock, kStreamFeatures, true)) return st;
+  op.token_rows = static_cast<int>(p.m);
+  op.whole = p.k % kBlock == 0;
+  const int scale_rows = std::min(kStreamWarps, p.num_kb);
+  op.scale_bytes = scale_rows * kStreamTokens * 4;
+  if (int st = make_map(&op.tm_scale, p.a_scales, 4, p.m, p.num_kb, kStreamTokens, scale_rows,
+                        false, p.a_pitch)) {
+    return st;
+  }
+  if (int st = op.tokens.make(p.a, 1, p.k, p.m, op.token_rows, kStreamWarps, op.whole)) return st;
+  if (int st = op.w[0].make(p.b, 1, p.k, p.n, op.tiles.rows, kStreamWarps, op.whole)) return st;
+  if (int st = op.less[0].make(p.b, 1, p.k, p.n, std::max(1, op.tiles.rows - 1), kStreamWarps,
+                               op.whole)) {
+    return st;
+  }
   return launch_stream(op, p.after_quantise, s);
 }
 

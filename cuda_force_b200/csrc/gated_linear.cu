@@ -517,65 +517,42 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
 
 template <bool kBf16>
 struct GatedStreamOp {
-  CUtensorMap tm_w[2];
+  static constexpr int kMatrices = 2, kBlocks = kStreamBlocks, kBlockElems = kDepth;
+  static constexpr int kScaleBytes = 0;
+  struct Weights {};
+
+  StreamMap w[2], less[2], tokens;
   GatedParams p;
   float *gate, *up;  // g and u for the backward pass, or null
   unsigned *err;
-  int tiles, steps;
+  StreamTiles tiles;
+  int steps, blocks, token_rows, scale_bytes;
+  bool whole;
 
-  struct Tokens {
-    uint4 x[2];
-  };
+  __device__ __forceinline__ void load_scales(uint8_t *, uint64_t *, int) const {}
+  __device__ __forceinline__ void fetch(Weights &, int, int, int) const {}
 
-  __device__ __forceinline__ void begin() const {}
-
-  __device__ __forceinline__ unsigned boxes(int step) const {
-    const unsigned half = (1u << min(kStreamBlocks, p.num_kb - step * kStreamBlocks)) - 1u;
-    return half | half << kStreamBlocks;
-  }
-
-  __device__ __forceinline__ void load_box(uint8_t *dst, uint64_t *bar, int tile, int step,
-                                           int box) const {
-    ptx::tma_load_2d(dst, &tm_w[box / kStreamBlocks], bar,
-                     (step * kStreamBlocks + box % kStreamBlocks) * kDepth,
-                     tile * kStreamFeatures);
-  }
-
-  __device__ __forceinline__ void load(Tokens &l, int tile, int step, int warp) const {
-    const int kb = step * kStreamBlocks + warp % kStreamBlocks;
-    if (kb >= p.num_kb || tile >= tiles) return;
-    const int lane = threadIdx.x % kWarp, g = lane / 4, t = lane % 4;
-    const int64_t k = static_cast<int64_t>(kb) * kDepth + t * 16;
-    const uint4 *src =
-        reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.x) + g * p.k + k);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {  // k is a multiple of 8: all 16 bytes or none
-      l.x[h] = g < p.m && k + 8 * h < p.k ? __ldg(src + h) : make_uint4(0, 0, 0, 0);
-    }
-  }
-
-  __device__ __forceinline__ void multiply(const StreamRows &r, const Tokens &l,
+  __device__ __forceinline__ void multiply(const StreamRows &r, const uint4 (&x)[2],
+                                           const float (&)[2], const Weights &, int, int,
                                            float (&acc)[4]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      mma_16x8x16<kBf16>(acc, r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, l.x[h].x,
-                         l.x[h].y);
-      mma_16x8x16<kBf16>(acc, r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, l.x[h].z,
-                         l.x[h].w);
+      mma_16x8x16<kBf16>(acc, r.w[0][h].x, r.w[1][h].x, r.w[0][h].y, r.w[1][h].y, x[h].x, x[h].y);
+      mma_16x8x16<kBf16>(acc, r.w[0][h].z, r.w[1][h].z, r.w[0][h].w, r.w[1][h].w, x[h].z, x[h].w);
     }
   }
 
-  __device__ __forceinline__ void store(int tile, const float *red) const {
+  __device__ __forceinline__ void store(int feature, int count, const float *red) const {
     if (threadIdx.x >= kStreamTokens * kStreamFeatures) return;
     const int m = threadIdx.x / kStreamFeatures, f = threadIdx.x % kStreamFeatures;
-    const int64_t n = static_cast<int64_t>(tile) * kStreamFeatures + f;
+    const int64_t n = int64_t{feature} + f;
     float g = 0.0f, u = 0.0f;
 #pragma unroll
     for (int w = 0; w < kStreamBlocks; ++w) {
       g += red[(w * kStreamTokens + m) * kStreamRedRow + f];
       u += red[((w + kStreamBlocks) * kStreamTokens + m) * kStreamRedRow + f];
     }
-    if (m < p.m && n < p.n) {
+    if (m < p.m && f < count && n < p.n) {
       const int64_t at = m * p.n + n;
       const float v = g * gate_sigmoid(g, p.act) * u;
       static_cast<uint16_t *>(p.y)[at] = static_cast<uint16_t>(pack2<kBf16>(v, 0.0f));
@@ -595,14 +572,21 @@ int launch_gated_stream(const GatedParams &p, float *gate, float *up, cudaStream
   op.up = up;
   op.err = device_error_word();
   if (op.err == nullptr) return record_cuda_error(cudaGetLastError());
-  op.tiles = static_cast<int>((p.n + kStreamFeatures - 1) / kStreamFeatures);
+  op.tiles = stream_tiles(p.n);
+  op.blocks = p.num_kb;
   op.steps = (p.num_kb + kStreamBlocks - 1) / kStreamBlocks;
+  op.token_rows = static_cast<int>(p.m);
+  op.scale_bytes = 0;
+  op.whole = p.k % kDepth == 0;
   const void *w[2] = {p.w_gate, p.w_up};
-  for (int i = 0; i < 2; ++i) {
-    if (int st = make_map(&op.tm_w[i], w[i], 2, p.k, p.n, kDepth, kStreamFeatures, true)) {
-      return st;
-    }
+  int st = op.tokens.make(p.x, 2, p.k, p.m, op.token_rows, kStreamBlocks, op.whole);
+  for (int i = 0; i < 2 && st == CF_OK; ++i) {
+    st = op.w[i].make(w[i], 2, p.k, p.n, op.tiles.rows, kStreamBlocks, op.whole);
+    if (st != CF_OK) break;
+    st = op.less[i].make(w[i], 2, p.k, p.n, std::max(1, op.tiles.rows - 1), kStreamBlocks,
+                         op.whole);
   }
+  if (st != CF_OK) return st;
   return launch_stream(op, false, s);
 }
 

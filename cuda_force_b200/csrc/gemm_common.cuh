@@ -161,24 +161,45 @@ inline CUtensorMapSwizzle swizzle_for(int inner_bytes) {
   }
 }
 
+inline int encode_map(CUtensorMap *map, const void *base, int esize, int rank,
+                      const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                      bool swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return record_cuda_error(cudaErrorNotSupported);
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = esize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  const CUresult r =
+      fn(map, dt, static_cast<cuuint32_t>(rank), const_cast<void *>(base), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE,
+         swizzle ? swizzle_for(static_cast<int>(box[0]) * esize) : CU_TENSOR_MAP_SWIZZLE_NONE,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CF_OK : CF_ERR_UNSUPPORTED;
+}
+
 // 2-D row-major tensor [outer, inner] with element size esize and rows `ld` elements apart
 // (0: inner), box [box_outer, box_inner].
 inline int make_map(CUtensorMap *map, const void *base, int esize, int64_t inner, int64_t outer,
                     int box_inner, int box_outer, bool swizzle, int64_t ld = 0) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return record_cuda_error(cudaErrorNotSupported);
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld ? ld : inner) * esize};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapDataType dt = esize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                 : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
-                                              : CU_TENSOR_MAP_DATA_TYPE_UINT32;
-  const CUresult r = fn(map, dt, 2, const_cast<void *>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle ? swizzle_for(box_inner * esize) : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? CF_OK : CF_ERR_UNSUPPORTED;
+  return encode_map(map, base, esize, 2, dims, strides, box, swizzle);
+}
+
+// The same tensor, rows of whole 128-byte blocks, as [block][row][128 bytes]: a box of
+// box_blocks blocks of box_rows rows, swizzled, in one copy.
+inline int make_block_map(CUtensorMap *map, const void *base, int esize, int64_t inner,
+                          int64_t outer, int box_rows, int box_blocks) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(128 / esize),
+                              static_cast<cuuint64_t>(outer),
+                              static_cast<cuuint64_t>(inner * esize / 128)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(inner) * esize, 128};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esize),
+                             static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(box_blocks)};
+  return encode_map(map, base, esize, 3, dims, strides, box, true);
 }
 
 }  // namespace
