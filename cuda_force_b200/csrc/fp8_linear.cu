@@ -389,8 +389,7 @@ struct Fp8StreamOp {
   Fp8Params p;
   unsigned *err;
   StreamTiles tiles;
-  int steps, blocks, token_rows, scale_bytes;
-  bool whole;
+  int steps, whole_steps, blocks, token_rows, scale_bytes;
 
   __device__ __forceinline__ void load_scales(uint8_t *dst, uint64_t *bar, int step) const {
     ptx::tma_load_2d(dst, &tm_scale, bar, 0, step * kStreamWarps);
@@ -453,17 +452,17 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
   op.blocks = p.num_kb;
   op.steps = (p.num_kb + kStreamWarps - 1) / kStreamWarps;
   op.token_rows = static_cast<int>(p.m);
-  op.whole = p.k % kBlock == 0;
+  op.whole_steps = stream_whole_steps(p.k, kStreamWarps);
   const int scale_rows = std::min(kStreamWarps, p.num_kb);
   op.scale_bytes = scale_rows * kStreamTokens * 4;
   if (int st = make_map(&op.tm_scale, p.a_scales, 4, p.m, p.num_kb, kStreamTokens, scale_rows,
                         false, p.a_pitch)) {
     return st;
   }
-  if (int st = op.tokens.make(p.a, 1, p.k, p.m, op.token_rows, kStreamWarps, op.whole)) return st;
-  if (int st = op.w[0].make(p.b, 1, p.k, p.n, op.tiles.rows, kStreamWarps, op.whole)) return st;
+  if (int st = op.tokens.make(p.a, 1, p.k, p.m, op.token_rows, kStreamWarps, op.whole_steps)) return st;
+  if (int st = op.w[0].make(p.b, 1, p.k, p.n, op.tiles.rows, kStreamWarps, op.whole_steps)) return st;
   if (int st = op.less[0].make(p.b, 1, p.k, p.n, std::max(1, op.tiles.rows - 1), kStreamWarps,
-                               op.whole)) {
+                               op.whole_steps)) {
     return st;
   }
   return launch_stream(op, p.after_quantise, s);

@@ -526,8 +526,7 @@ struct GatedStreamOp {
   float *gate, *up;  // g and u for the backward pass, or null
   unsigned *err;
   StreamTiles tiles;
-  int steps, blocks, token_rows, scale_bytes;
-  bool whole;
+  int steps, whole_steps, blocks, token_rows, scale_bytes;
 
   __device__ __forceinline__ void load_scales(uint8_t *, uint64_t *, int) const {}
   __device__ __forceinline__ void fetch(Weights &, int, int, int) const {}
@@ -577,14 +576,14 @@ int launch_gated_stream(const GatedParams &p, float *gate, float *up, cudaStream
   op.steps = (p.num_kb + kStreamBlocks - 1) / kStreamBlocks;
   op.token_rows = static_cast<int>(p.m);
   op.scale_bytes = 0;
-  op.whole = p.k % kDepth == 0;
+  op.whole_steps = stream_whole_steps(p.k * 2, kStreamBlocks);
   const void *w[2] = {p.w_gate, p.w_up};
-  int st = op.tokens.make(p.x, 2, p.k, p.m, op.token_rows, kStreamBlocks, op.whole);
+  int st = op.tokens.make(p.x, 2, p.k, p.m, op.token_rows, kStreamBlocks, op.whole_steps);
   for (int i = 0; i < 2 && st == CF_OK; ++i) {
-    st = op.w[i].make(w[i], 2, p.k, p.n, op.tiles.rows, kStreamBlocks, op.whole);
+    st = op.w[i].make(w[i], 2, p.k, p.n, op.tiles.rows, kStreamBlocks, op.whole_steps);
     if (st != CF_OK) break;
     st = op.less[i].make(w[i], 2, p.k, p.n, std::max(1, op.tiles.rows - 1), kStreamBlocks,
-                         op.whole);
+                         op.whole_steps);
   }
   if (st != CF_OK) return st;
   return launch_stream(op, false, s);

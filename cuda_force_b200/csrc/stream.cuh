@@ -74,17 +74,22 @@ inline StreamTiles stream_tiles(int64_t n) {
   return t;
 }
 
-// The tensor maps of one operand, [rows, k] in blocks of 128 bytes. `whole` (k is a
-// number of whole blocks): a stage's blocks of a tile's rows in one copy, [block][row];
-// the copies' number is what bounds these kernels otherwise (8 boxes of 16 x 128 bytes
-// a stage: 115 cycles a box, however many of its rows exist). Else a copy for each
-// block, `pitch` rows apart.
+// The tensor maps of one operand, [rows, k] in blocks of 128 bytes. The first
+// `whole_steps` stages come in one copy, [block][row]: the copies' number is what bounds
+// these kernels otherwise (eight boxes of 16 x 128 bytes a stage: 115 cycles a box,
+// however many of its rows exist). A last stage with part of a block, which such a map
+// cannot describe, takes a copy for each block, `pitch` rows apart.
 struct StreamMap {
-  CUtensorMap tm;
+  CUtensorMap tm, tm_block;
 
-  int make(const void *base, int esize, int64_t k, int64_t n, int rows, int blocks, bool whole) {
-    return whole ? make_block_map(&tm, base, esize, k, n, rows, blocks)
-                 : make_map(&tm, base, esize, k, n, 128 / esize, rows, true);
+  int make(const void *base, int esize, int64_t k, int64_t n, int rows, int blocks,
+           int whole_steps) {
+    int st = CF_OK;
+    if (whole_steps > 0) st = make_block_map(&tm, base, esize, k, n, rows, blocks);
+    if (st == CF_OK && k * esize % 128 != 0) {
+      st = make_map(&tm_block, base, esize, k, n, 128 / esize, rows, true);
+    }
+    return st;
   }
 
   // By a whole warp: block `block` and those after it, as the mask `exist` says.
@@ -95,15 +100,23 @@ struct StreamMap {
     if (whole) {
       if (lane == 0) ptx::tma_load_3d(dst, &tm, bar, 0, row, block);
     } else if (lane < kBlocks && (exist >> lane & 1u)) {
-      ptx::tma_load_2d(dst + lane * kPitch * 128, &tm, bar, (block + lane) * kBlockElems, row);
+      ptx::tma_load_2d(dst + lane * kPitch * 128, &tm_block, bar, (block + lane) * kBlockElems,
+                       row);
     }
   }
 };
 
+// Stages that are copied whole: all of them where k is whole blocks (what is beyond k is
+// zeros then).
+inline int stream_whole_steps(int64_t k_bytes, int blocks) {
+  return static_cast<int>(k_bytes % 128 == 0 ? (k_bytes / 128 + blocks - 1) / blocks
+                                             : k_bytes / 128 / blocks);
+}
+
 // Op: what is multiplied. kMatrices of weights share the warps, kBlocks of 128 bytes of
 // k (kBlockElems elements) a stage for each, of the same tokens. w[matrix] and
 // less[matrix], the maps of a tile's rows and of one row less, tokens, token_rows,
-// blocks (of k), whole; tiles, steps (stages of a tile), err. kScaleBytes of the tokens'
+// blocks (of k); tiles, steps (stages of a tile), whole_steps, err. kScaleBytes of the tokens'
 // scales by load_scales(dst, bar, step), scale_bytes of them copied, or none.
 // Weights, the weights' scales of a lane: fetch(weights, feature, step, warp) at every
 // 32nd step for the next 32, ahead of the tile; multiply(rows, token words, scales,
@@ -147,7 +160,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
       return (1u << min(Op::kBlocks, op.blocks - step * Op::kBlocks)) - 1u;
     };
     auto weights = [&] {
-      const int copied = op.whole ? Op::kBlocks : __popc(exist());  // zeros beyond the last
+      const int copied = step < op.whole_steps ? Op::kBlocks : __popc(exist());  // zeros beyond the last
       if (lane == 0) {
         ptx::mbar_expect_tx(&full[stage],
                             copied * (Op::kMatrices * count + op.token_rows) * 128 +
@@ -159,7 +172,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         (count < op.tiles.rows ? op.less[i] : op.w[i])
             .template load<Op::kBlocks, kStreamFeatures, Op::kBlockElems>(
                 smem + stage * C::kStageBytes + i * Op::kBlocks * kStreamBoxBytes, &full[stage],
-                feature, step * Op::kBlocks, exist(), op.whole);
+                feature, step * Op::kBlocks, exist(), step < op.whole_steps);
       }
       outstanding |= 1u << stage;
       parities = (parities & ~(1u << stage)) | (phase << stage);
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     auto tokens = [&] {
       op.tokens.template load<Op::kBlocks, kStreamTokens, Op::kBlockElems>(
           smem + stage * C::kStageBytes + kStreamWarps * kStreamBoxBytes, &full[stage], 0,
-          step * Op::kBlocks, exist(), op.whole);
+          step * Op::kBlocks, exist(), step < op.whole_steps);
       if constexpr (Op::kScaleBytes > 0) {
         if (lane == 0) {
           op.load_scales(smem + C::kScales + stage * Op::kScaleBytes, &full[stage], step);
@@ -237,8 +250,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         const uint32_t in_stage = base + stage * C::kStageBytes;
         const uint32_t tokens = in_stage + kStreamWarps * kStreamBoxBytes;
         const uint32_t weights = in_stage + (warp - block) * kStreamBoxBytes;
-        const int row = block * (op.whole ? count : kStreamFeatures) + g;
-        const int token = block * (op.whole ? op.token_rows : kStreamTokens) + g;
+        const int row = block * (step < op.whole_steps ? count : kStreamFeatures) + g;
+        const int token = block * (step < op.whole_steps ? op.token_rows : kStreamTokens) + g;
         StreamRows rows;
         uint4 x[2];
 #pragma unroll

@@ -149,6 +149,8 @@ SHAPES = [
     # few tiles: clusters of 2, 4 and 8 CTAs share a tile's k, ragged shares, odd features
     (40, 11008, 4096), (20, 1040, 2000), (100, 2064, 1031), (130, 4096, 200), (64, 8192, 64),
     (9, 4112, 7), (300, 1040, 129),
+    # streamed: one feature, tiles of two sizes, several to a CTA, more than 32 stages a tile
+    (1, 48, 1), (4, 144, 9), (6, 1024, 301), (7, 4224, 11008), (2, 33040, 600), (8, 32896, 2405),
 ]
 
 

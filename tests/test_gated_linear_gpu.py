@@ -82,6 +82,8 @@ SHAPES = [
     (1000, 504, 2056), (2500, 1024, 2048),
     # few tiles of dx: clusters of 2, 4 and 8 CTAs share its contraction
     (5, 264, 4104), (130, 1000, 2600), (200, 2048, 1200), (700, 520, 5000),
+    # streamed: tiles of two sizes, several to a CTA
+    (4, 256, 304), (2, 1000, 9608), (8, 576, 11008),
 ]
 
 
