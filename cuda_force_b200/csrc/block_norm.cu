@@ -1070,7 +1070,6 @@ int threads_per_row(int64_t cols, int per) {
   return 0;
 }
 
-
 // The longest row of the staged and simple backward kernels.
 constexpr int64_t kBackwardMaxCols = 8192;
 

@@ -181,9 +181,9 @@ constexpr int kQuantUnroll = sizeof(T) == 4 ? 2 : 4;
 
 // 1 x 128 blocks: 16 lanes a block, eight elements a lane; kUnroll blocks a
 // half-warp, loaded before any is reduced. [8192, 11008] bf16: 58 us, 4.6 TB/s,
-// bound by instruction issue (fp32, half the instructions a byte: 5.8). Everything beyond a CTA's first block
-// is 32-bit offsets: at 16 bits an element 64-bit addresses were a third of the
-// instructions, and their registers half of the CTAs that fit on an SM.
+// bound by instruction issue (fp32, half the instructions a byte: 5.8). Everything beyond
+// a CTA's first block is 32-bit offsets: at 16 bits an element 64-bit addresses were a
+// third of the instructions, and their registers half of the CTAs that fit on an SM.
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kQuantThreads, 4)
     fp8_quantize_rows_kernel(const T *x, uint8_t *codes, float *scales, int64_t blocks, int cols,
@@ -364,8 +364,8 @@ struct Fp8Params {
   unsigned *err;
 };
 
-// Few rows: the streaming kernel with m16n8k32 on e4m3, a box is 16 features of
-// one 128-block of k and a stage eight such blocks.
+// Few rows: the streaming kernel with m16n8k32 on e4m3, a block is one of the
+// scales' 128 elements of k.
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 "
@@ -459,12 +459,12 @@ int launch_fp8_stream(const Fp8Params &p, cudaStream_t s) {
                         false, p.a_pitch)) {
     return st;
   }
-  if (int st = op.tokens.make(p.a, 1, p.k, p.m, op.token_rows, kStreamWarps, op.whole_steps)) return st;
-  if (int st = op.w[0].make(p.b, 1, p.k, p.n, op.tiles.rows, kStreamWarps, op.whole_steps)) return st;
-  if (int st = op.less[0].make(p.b, 1, p.k, p.n, std::max(1, op.tiles.rows - 1), kStreamWarps,
-                               op.whole_steps)) {
-    return st;
-  }
+  auto map = [&](StreamMap &to, const uint8_t *base, int64_t n, int rows) {
+    return to.make(base, 1, p.k, n, rows, kStreamWarps, op.whole_steps);
+  };
+  if (int st = map(op.tokens, p.a, p.m, op.token_rows)) return st;
+  if (int st = map(op.w[0], p.b, p.n, op.tiles.rows)) return st;
+  if (int st = map(op.less[0], p.b, p.n, std::max(1, op.tiles.rows - 1))) return st;
   return launch_stream(op, p.after_quantise, s);
 }
 

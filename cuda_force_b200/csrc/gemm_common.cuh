@@ -184,7 +184,8 @@ inline int make_map(CUtensorMap *map, const void *base, int esize, int64_t inner
                     int box_inner, int box_outer, bool swizzle, int64_t ld = 0) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld ? ld : inner) * esize};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner),
+                             static_cast<cuuint32_t>(box_outer)};
   return encode_map(map, base, esize, 2, dims, strides, box, swizzle);
 }
 

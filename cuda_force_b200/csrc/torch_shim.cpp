@@ -426,7 +426,8 @@ std::vector<at::Tensor> gated_residual_rmsnorm_cuda(
 // Gradients of x, residual, weight, post_weight and gate in their own dtypes; an
 // absent parameter's is undefined.
 std::vector<at::Tensor> block_norm_backward(
-    at::Tensor dn, at::Tensor dh, const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight,
+    at::Tensor dn, at::Tensor dh, const at::Tensor &x, const at::Tensor &residual,
+    const at::Tensor &weight,
     const std::optional<at::Tensor> &post_weight, const std::optional<at::Tensor> &gate,
     int64_t gate_groups, double residual_scale, const at::Tensor &stats) {
   check_cuda(x, "x");
