@@ -647,7 +647,9 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
 #pragma unroll
     for (int e = 0; e < kPairs; ++e) sum_w[i][e] = sum_p[i][e] = sum_g[i][e] = both(0.0f);
   }
-  float2 stats = begin < end ? reinterpret_cast<const float2 *>(a.stats)[begin] : float2{};
+  // Two loads: a caller's stats need no more than a float's alignment.
+  auto stats_of = [&](int64_t row) { return make_float2(a.stats[2 * row], a.stats[2 * row + 1]); };
+  float2 stats = begin < end ? stats_of(begin) : float2{};
   const Pair scale2 = both(a.scale);
 
   for (int64_t row = begin; row < end; ++row) {
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
                                        : static_cast<const TW *>(a.gate) +
                                              (kShared ? row / a.gate_rows : row) * a.cols;
     const Pair q2 = both(stats.x), rt2 = both(stats.y);
-    if (row + 1 < end) stats = reinterpret_cast<const float2 *>(a.stats)[row + 1];
+    if (row + 1 < end) stats = stats_of(row + 1);
     ring.wait();
     const T *x = ring.template row<T>(0);
     const T *r = ring.template row<T>(1);
