@@ -50,7 +50,9 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 
 // Eight elements to eight codes. fl32(x / s) without a division, two at a time: r
 // = fl32(1 / s), q0 = fl(x r), the exact residual and Markstein's correction step
-// (as quant_math.cuh).
+// (as quant_math.cuh). The residual is rounded downwards, which being exact it does
+// not notice, except that a zero is -0 then: added to q0 = -0, the quotient of x = -0,
+// a +0 would lose the sign.
 __device__ __forceinline__ uint2 fp8_codes(const float (&f)[8], float s, float r, bool fast) {
   float q[8];
   if (fast) {
@@ -59,7 +61,8 @@ __device__ __forceinline__ uint2 fp8_codes(const float (&f)[8], float s, float r
     for (int i = 0; i < 4; ++i) {
       const uint64_t x2 = ptx::pack_f32x2(f[2 * i], f[2 * i + 1]);
       const uint64_t q0 = ptx::mul_f32x2(x2, r2);
-      const float2 v = ptx::unpack_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(q0, neg_s2, x2), r2, q0));
+      const float2 v =
+          ptx::unpack_f32x2(ptx::fma_f32x2(ptx::fma_down_f32x2(q0, neg_s2, x2), r2, q0));
       q[2 * i] = v.x;
       q[2 * i + 1] = v.y;
     }
