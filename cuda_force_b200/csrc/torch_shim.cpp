@@ -543,6 +543,13 @@ std::vector<at::Tensor> gated_residual_rmsnorm_autograd(
 
 // ---- gated projections
 
+// Rows of x, whatever its last dimension: also where that is 0.
+int64_t token_rows(const at::Tensor &x) {
+  int64_t m = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
+  return m;
+}
+
 // A copy where the kernels' 16-byte alignment is not met (a slice of a larger tensor).
 at::Tensor aligned16(const at::Tensor &t) {
   return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
@@ -565,7 +572,7 @@ std::vector<at::Tensor> gated_forward(const at::Tensor &x, const at::Tensor &w_g
                 " must have x's dtype and device");
   }
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t k = x.size(-1), n = w_gate.size(0), m = k > 0 ? x.numel() / k : 0;
+  const int64_t k = x.size(-1), n = w_gate.size(0), m = token_rows(x);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
   std::vector<at::Tensor> out{at::empty(shape, x.options())};
@@ -576,6 +583,10 @@ std::vector<at::Tensor> gated_forward(const at::Tensor &x, const at::Tensor &w_g
     }
     gate = out[1].data_ptr<float>();
     up = out[2].data_ptr<float>();
+  }
+  if (k == 0) {  // empty sums
+    for (at::Tensor &t : out) t.zero_();
+    return out;
   }
   const at::Tensor xa = aligned16(x), wg = aligned16(w_gate), wu = aligned16(w_up);
   check_status(cf_gated_linear(xa.const_data_ptr(), wg.const_data_ptr(), wu.const_data_ptr(),
@@ -735,9 +746,7 @@ at::Tensor linear_fp8_cuda(const at::Tensor &x, const at::Tensor &w_codes,
   const int dtype = dtype_code(x, "x");
   TORCH_CHECK(dtype != CF_DTYPE_F32, "linear_fp8: x must be bfloat16 or float16");
   TORCH_CHECK(x.device() == w_codes.device(), "x and w must share a device");
-  const int64_t k = x.size(-1), n = w_codes.size(0);
-  int64_t m = 1;
-  for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
+  const int64_t k = x.size(-1), n = w_codes.size(0), m = token_rows(x);
   TORCH_CHECK(w_codes.size(1) == k, "w codes must be [n, ", k, "], got ", w_codes.sizes());
   const c10::cuda::CUDAGuard guard(x.device());
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
