@@ -29,7 +29,7 @@ SHIM = PKG / "_C.so"
 CUDA_SOURCES = ["abi.cu", "quant.cu", "lora_gemm.cu", "norm.cu", "block_norm.cu",
                 "fp8_linear.cu", "gated_linear.cu"]
 HEADERS = ["quant_math.cuh", "cf_common.cuh", "ptx.cuh", "gemm_common.cuh", "row_ring.cuh",
-           "stream.cuh"]
+           "stage_ring.cuh", "stream.cuh"]
 
 NVCC_FLAGS = [
     "-O3",

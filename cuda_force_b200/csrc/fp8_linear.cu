@@ -19,6 +19,7 @@
 #include "cf_common.cuh"
 #include "gemm_common.cuh"
 #include "ptx.cuh"
+#include "stage_ring.cuh"
 #include "stream.cuh"
 
 namespace cfb {
@@ -589,52 +590,43 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
       ptx::grid_dep_wait();  // the tokens' codes and scales
-      int stage = 0, slot = 0;
-      uint32_t phase = 0, outstanding = 0, parities = 0;
+      StageRing<C::kStages> ring;
+      int slot = 0;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
         int tm, tn;
         band_order(tile, p.m_tiles, p.n_tiles, p.band, tm, tn);
         const int a_row = (tm * kCtas + static_cast<int>(rank)) * kTileM;
         const int b_row = tn * kN + static_cast<int>(rank) * C::kBRows;
         for (int kb = kb_begin; kb < kb_end; ++kb) {
-          if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
+          if (!ring.wait_free(empty)) {
             record_timeout(p.err, abort_flag);
             break;
           }
-          uint8_t *sa = smem + stage * C::kOperandBytes;
+          uint64_t *const landed = &full[ring.stage];
+          uint8_t *sa = smem + ring.stage * C::kOperandBytes;
           uint8_t *scale = smem + C::kScaleOffset + slot * C::kScaleBytes;
           const uint32_t bytes =
               C::kOperandBytes + C::kScaleBytes - (kTileM - p.a_rows) * kBlock;
           if constexpr (kCtas == 2) {
             // The even CTA's barrier counts both CTAs' bytes.
-            const uint32_t bar = ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0);
-            if (rank == 0) ptx::mbar_expect_tx(&full[stage], 2 * bytes);
+            const uint32_t bar = ptx::map_shared_rank(ptx::smem_addr(landed), 0);
+            if (rank == 0) ptx::mbar_expect_tx(landed, 2 * bytes);
             ptx::tma_load_2d_pair(sa, &tm_a, bar, kb * kBlock, a_row);
             ptx::tma_load_2d_pair(sa + C::kABytes, &tm_b, bar, kb * kBlock, b_row);
             ptx::tma_load_2d_pair(scale, &tm_scale, bar, a_row, kb);
           } else {
-            ptx::mbar_expect_tx(&full[stage], bytes);
-            ptx::tma_load_2d(sa, &tm_a, &full[stage], kb * kBlock, a_row);
-            ptx::tma_load_2d(sa + C::kABytes, &tm_b, &full[stage], kb * kBlock, b_row);
-            ptx::tma_load_2d(scale, &tm_scale, &full[stage], a_row, kb);
+            ptx::mbar_expect_tx(landed, bytes);
+            ptx::tma_load_2d(sa, &tm_a, landed, kb * kBlock, a_row);
+            ptx::tma_load_2d(sa + C::kABytes, &tm_b, landed, kb * kBlock, b_row);
+            ptx::tma_load_2d(scale, &tm_scale, landed, a_row, kb);
           }
-          outstanding |= 1u << stage;
-          parities = (parities & ~(1u << stage)) | (phase << stage);
+          ring.filled();
           if (++slot == C::kScaleSlots) slot = 0;
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
       }
-      if (aborted(abort_flag) && rank == 0) {
-        // Let loads in flight (both CTAs' count here) land before the end.
-        for (int s = 0; s < C::kStages; ++s) {
-          if (outstanding & (1u << s)) {
-            ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
-          }
-        }
-      }
+      if (!aborted(abort_flag) && !ring.wait_all_free(empty)) record_timeout(p.err, abort_flag);
+      // Let loads in flight (both CTAs' count here) land before the end.
+      if (aborted(abort_flag) && rank == 0) ring.drain(full);
     }
   } else if (warp == C::kEpilogueWarps + 1) {
     // ------------------------------------------------------------------ MMA issuer
@@ -689,7 +681,7 @@ __global__ void __launch_bounds__(TileCfg<kCtas, kN>::kThreads, 1)
       if (aborted(abort_flag)) {
         if (issuer) {
           if constexpr (kCtas == 2) {
-            ptx::mma_commit_pair(drain);
+            ptx::mma_commit_leader(drain);
           } else {
             ptx::mma_commit(drain);
           }

@@ -30,6 +30,7 @@
 #include "cf_common.cuh"
 #include "gemm_common.cuh"
 #include "ptx.cuh"
+#include "stage_ring.cuh"
 #include "stream.cuh"
 
 namespace cfb {
@@ -176,31 +177,31 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   if (warp == 8) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, outstanding = 0, parities = 0;
+      StageRing<C::kStages> ring;
       for (int tile = first; tile < tiles && !aborted(abort_flag); tile += step) {
         const int which = kMode == kWeights ? tile / per_matrix : 0;
         int tm, tn;
         band_order(tile - which * per_matrix, p.m_tiles, p.n_tiles, p.band, tm, tn);
         const int row = (tm * kCtas + rank) * kTileRows;
         for (int kb = kb_begin; kb < kb_end; ++kb) {
-          if (!ptx::mbar_wait(&empty[stage], phase ^ 1)) {
+          if (!ring.wait_free(empty)) {
             record_timeout(p.err, abort_flag);
             break;
           }
-          uint8_t *sa = smem + stage * C::kStageBytes;
+          uint64_t *const landed = &full[ring.stage];
+          uint8_t *sa = smem + ring.stage * C::kStageBytes;
           uint8_t *sb = sa + C::kABytes;
           // The even CTA's barrier counts both CTAs' bytes.
-          const uint32_t bar = kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(&full[stage]), 0)
-                                          : ptx::smem_addr(&full[stage]);
+          const uint32_t bar = kCtas == 2 ? ptx::map_shared_rank(ptx::smem_addr(landed), 0)
+                                          : ptx::smem_addr(landed);
           const uint32_t bytes =
               kMode == kWeights ? C::kStageBytes : C::kStageBytes - (kTileRows - p.a_rows) * 128;
-          if (rank == 0) ptx::mbar_expect_tx(&full[stage], kCtas * bytes);
+          if (rank == 0) ptx::mbar_expect_tx(landed, kCtas * bytes);
           auto load = [&](uint8_t *dst, const CUtensorMap *map, int c0, int c1) {
             if constexpr (kCtas == 2) {
               ptx::tma_load_2d_pair(dst, map, bar, c0, c1);
             } else {
-              ptx::tma_load_2d(dst, map, &full[stage], c0, c1);
+              ptx::tma_load_2d(dst, map, landed, c0, c1);
             }
           };
           // MN-major: chunks of 64 columns (one swizzle row) x 64 contracted rows.
@@ -234,22 +235,12 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
               }
             }
           }
-          outstanding |= 1u << stage;
-          parities = (parities & ~(1u << stage)) | (phase << stage);
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          ring.filled();
         }
       }
-      if (aborted(abort_flag) && rank == 0) {
-        // Let loads in flight (both CTAs' count here) land before the end.
-        for (int s = 0; s < C::kStages; ++s) {
-          if (outstanding & (1u << s)) {
-            ptx::mbar_wait(&full[s], (parities >> s) & 1u, 200000000ull);
-          }
-        }
-      }
+      if (!aborted(abort_flag) && !ring.wait_all_free(empty)) record_timeout(p.err, abort_flag);
+      // Let loads in flight (both CTAs' count here) land before the end.
+      if (aborted(abort_flag) && rank == 0) ring.drain(full);
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA issuer
@@ -319,7 +310,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       if (aborted(abort_flag)) {
         if (issuer) {
           if constexpr (kCtas == 2) {
-            ptx::mma_commit_pair(drain);
+            ptx::mma_commit_leader(drain);
           } else {
             ptx::mma_commit(drain);
           }

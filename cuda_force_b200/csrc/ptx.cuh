@@ -340,6 +340,14 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
       : "memory");
 }
 
+// The same on the issuing CTA's `bar` alone.
+__device__ __forceinline__ void mma_commit_leader(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
+
 // Tile of this CTA's operands, into its own shared memory; completes on the
 // barrier at `bar_addr`, a shared::cluster address in either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map,
