@@ -178,6 +178,8 @@ __device__ __forceinline__ void store8(uint8_t *p, int left, uint2 codes) {
 }
 
 constexpr int kQuantThreads = 256;
+// Longest row: a CTA's offsets from its first row are 32-bit.
+constexpr int64_t kQuantMaxCols = int64_t{1} << 30;
 // Blocks in flight for each half-warp (at [8192, 4096] fp32, two: 29 us, four: 33;
 // at [8192, 11008] bf16, two: 63, four: 58).
 template <typename T>
@@ -951,7 +953,7 @@ int cf_quantize_fp8(const void *input, int dtype, uint8_t *codes, float *scales,
   if (block_rows != 1 && block_rows != CF_FP8_BLOCK_SIZE) return CF_ERR_UNSUPPORTED;
   if (rows == 0 || cols == 0) return CF_OK;
   if (!input || !codes || !scales) return CF_ERR_INVALID_ARGUMENT;
-  if (rows > (int64_t{1} << 40) / cols || cols > (int64_t{1} << 30)) {
+  if (rows > (int64_t{1} << 40) / cols || cols > cfb::kQuantMaxCols) {
     return CF_ERR_INVALID_ARGUMENT;
   }
   return cfb::quantize_fp8_any(input, dtype, codes, scales, rows, cols, block_rows, 0,
@@ -988,7 +990,9 @@ int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, 
                   cf_stream_t stream) {
   if (int st = cfb::check_fp8_shape(m, k, n, dtype)) return st;
   if (m == 0 || n == 0) return CF_OK;
-  if (!x || !w_codes || !w_scales || !y) return CF_ERR_INVALID_ARGUMENT;
+  if (!x || !w_codes || !w_scales || !y || k > cfb::kQuantMaxCols) {
+    return CF_ERR_INVALID_ARGUMENT;
+  }
   if (!cfb::aligned_to(x, 16) || !cfb::aligned_to(w_codes, 16) || !cfb::aligned_to(y, 16)) {
     return CF_ERR_MISALIGNED;
   }

@@ -367,7 +367,7 @@ CF_API int cf_gated_linear_backward(const void *dy, const void *x, const void *w
  * blocks of block_rows (1 or CF_FP8_BLOCK_SIZE) x CF_FP8_BLOCK_SIZE elements:
  *   scale = fl32(absmax * fl32(1 / 448)), replaced by 1 when it is not > 0
  *   code  = e4m3(fl32(x / scale)), nearest even, saturating, NaN kept
- * Blocks at the end of a row or column may be smaller. codes: one byte each,
+ * Blocks at the end of a row or column may be smaller. cols <= 2^30. codes: one byte each,
  * [rows, cols]; scales: float [ceil(rows / block_rows)][ceil(cols / 128)]. Any
  * alignment works; a 16-byte aligned input, 8-byte aligned codes and cols % 8 ==
  * 0 take the vector path. No counterpart in the reference. */
@@ -388,7 +388,7 @@ CF_API int cf_matmul_fp8(const uint8_t *a_codes, const float *a_scales, int64_t 
 /* cf_quantize_fp8 of x [m, k] (dtype f16 or bf16) in blocks of 1 x 128, then
  * cf_matmul_fp8 with the weight w [n, k] (nn.Linear layout), which may begin while
  * the first still runs. The codes and scales of x go to `workspace`
- * (cf_linear_fp8_workspace_bytes, 16-byte aligned). x 16-byte aligned. */
+ * (cf_linear_fp8_workspace_bytes, 16-byte aligned). x 16-byte aligned, k <= 2^30. */
 CF_API size_t cf_linear_fp8_workspace_bytes(int64_t m, int64_t k);
 CF_API int cf_linear_fp8(const void *x, const uint8_t *w_codes, const float *w_scales, void *y,
                          int64_t m, int64_t k, int64_t n, int dtype, void *workspace,
