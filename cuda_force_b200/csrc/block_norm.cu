@@ -1186,7 +1186,9 @@ int dispatch_norm(const NormArgs &a, int dtype, int weight_dtype, bool wide, voi
 // Checks shared by both directions.
 int check_norm_args(int64_t rows, int64_t cols, int64_t gate_groups, bool gate, int dtype,
                     int weight_dtype) {
-  if (rows < 0 || cols < 0 || gate_groups < (rows > 0 ? 1 : 0)) return CF_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || cols < 0 || (gate && gate_groups < (rows > 0 ? 1 : 0))) {
+    return CF_ERR_INVALID_ARGUMENT;
+  }
   if (dtype != CF_DTYPE_F32 && dtype != CF_DTYPE_BF16 && dtype != CF_DTYPE_F16) {
     return CF_ERR_UNSUPPORTED;
   }

@@ -299,12 +299,13 @@ CF_API int cf_fused_residual_rmsnorm(const void *x, const void *residual, const 
  * in fp32; residual_out = h and normalised are each rounded once to dtype
  * (normalised from the unrounded h). gate is [gate_groups, cols]: group g holds
  * rows [g * rows / gate_groups, ...), so 1 is a gate for each channel and rows a
- * gate for each element; rows % gate_groups == 0. weight, post_weight and gate
- * are of weight_dtype, which is dtype or f32. stats, float [rows][2], receives
- * what the backward pass needs, or is NULL. Any alignment works; 16-byte aligned
- * pointers and rows of whole 16-byte units take the vector path. No counterpart
- * in the reference, whose fused_residual_rmsnorm (cuda/include/cudaforge/
- * fused_norm.cuh) has neither post-norm, gate, scale nor a backward pass. */
+ * gate for each element; rows % gate_groups == 0 (not looked at when gate is
+ * NULL). weight, post_weight and gate are of weight_dtype, which is dtype or f32.
+ * stats, float [rows][2], receives what the backward pass needs, or is NULL. Any
+ * alignment of the elements works; 16-byte aligned tensors and rows of whole
+ * 16-byte units take the vector path. No counterpart in the reference, whose
+ * fused_residual_rmsnorm (cuda/include/cudaforge/fused_norm.cuh) has neither
+ * post-norm, gate, scale nor a backward pass. */
 CF_API int cf_gated_residual_rmsnorm(const void *x, const void *residual, const void *weight,
                                      const void *post_weight, const void *gate,
                                      int64_t gate_groups, int weight_dtype, void *normalised,

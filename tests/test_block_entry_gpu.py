@@ -66,3 +66,18 @@ def test_norm_statistics_on_a_four_byte_boundary(shape, dtype, cuda_device):
         results.append([*out, *norm_backward(x, residual, weight, post, gate, 1, dn, dh, stats)])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("rows, cols", [(7, 256), (6, 333), (3, 9000)])
+def test_norm_without_a_gate_has_no_gate_groups(rows, cols, cuda_device):
+    # 0, which the workspace's size takes for no gate, and any other number.
+    (x, residual, dn, dh), (weight, post, _) = norm_inputs(rows, cols, torch.float32, cuda_device)
+    results = []
+    for groups in (1, 0, -1, 5):
+        stats = torch.empty(rows, 2, device=cuda_device)
+        out = norm_forward(x, residual, weight, post, None, groups, stats)
+        results.append([*out, *norm_backward(x, residual, weight, post, None, groups, dn, dh,
+                                             stats)])
+    torch.cuda.synchronize()
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
