@@ -532,8 +532,8 @@ __device__ __forceinline__ void load_staged(const float *w, int c, int cols,
 // group's registers exactly, so no chunk is conditional; the branches around them
 // keep the compiler from interleaving the chunks. [8192, 4096] bf16 with a gate:
 // 91 us (105 with the branches, 157 without the ring), 4.4 TB/s, and 8 us to add
-// the partial sums; bound by instruction issue and latency at the 512 threads an
-// SM has registers for.
+// the partial sums; bound by latency at the 512 threads that an SM has registers
+// for (half of the issue slots are taken, and two thirds of the memory's rate).
 template <typename T, typename TW, int kTpr, bool kShared, bool kFull>
 __global__ void __launch_bounds__(cta_threads<kTpr>(), backward_ctas<kTpr>())
     gated_norm_backward_kernel(const NormArgs a) {

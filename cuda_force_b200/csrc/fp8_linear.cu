@@ -186,8 +186,10 @@ template <typename T>
 constexpr int kQuantUnroll = sizeof(T) == 4 ? 2 : 4;
 
 // 1 x 128 blocks: 16 lanes a block, eight elements a lane; kUnroll blocks a
-// half-warp, loaded before any is reduced. [8192, 11008] bf16: 58 us, 4.6 TB/s,
-// bound by instruction issue (fp32, half the instructions a byte: 5.8). Everything beyond
+// half-warp, loaded before any is reduced. [8192, 11008] bf16: 58 us, 4.6 TB/s, bound
+// by latency at the 1024 threads that an SM has registers for, a warp's loads and its
+// arithmetic taking turns (two thirds of the issue slots are taken, and of the memory's
+// rate; fp32, half the instructions a byte: 5.8). Everything beyond
 // a CTA's first block is 32-bit offsets: at 16 bits an element 64-bit addresses were a
 // third of the instructions, and their registers half of the CTAs that fit on an SM.
 template <typename T, bool kWide>

@@ -408,17 +408,6 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "r"(taddr));
 }
 
-// 32 lanes x 16 columns into exactly 16 registers.
-__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -462,10 +451,10 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   return r;
 }
 
-// All threads of all CTAs of the cluster; release/acquire orders shared-memory
-// writes before the barrier with distributed shared-memory reads after it.
-// Cluster-wide barrier. The .aligned forms require every thread of a warp to
-// execute them together, so the warp reconverges first.
+// Barrier over all threads of all CTAs of the cluster; release/acquire orders
+// shared-memory writes before it with distributed shared-memory reads after it.
+// The .aligned forms require every thread of a warp to execute them together, so the
+// warp reconverges first.
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" :::
@@ -570,7 +559,7 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
          ((static_cast<uint32_t>(m) >> 4) << 24);
 }
 
-// Both lanes of a packed f32x2 set to v.
+// Packed pairs of fp32, each lane as the scalar instruction.
 __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -609,6 +598,7 @@ __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
   return r;
 }
 
+// Both lanes set to v.
 __device__ __forceinline__ uint64_t splat_f32x2(float v) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
