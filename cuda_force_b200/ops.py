@@ -256,10 +256,10 @@ def gated_residual_rmsnorm(
 
     Args:
         x, residual: ``[..., hidden]`` of one float dtype.
-        weight, post_weight: ``[hidden]`` of any float dtype.
-        gate: ``[hidden]``, x's shape, or x's shape with trailing dimensions
-            before the last set to 1 (``[batch, 1, hidden]``: a gate for each
-            sample of ``[batch, tokens, hidden]``).
+        weight, post_weight: ``[hidden]``, float32, float16 or bfloat16.
+        gate: in one of those dtypes, ``[hidden]``, x's shape, or x's shape with
+            trailing dimensions before the last set to 1 (``[batch, 1, hidden]``: a
+            gate for each sample of ``[batch, tokens, hidden]``).
         residual_scale: a number.
 
     Differentiable in every tensor, once. Gradients of ``weight``,
@@ -605,8 +605,11 @@ def gated_linear(
         activation: ``"silu"``, or ``"gelu"`` in its tanh form.
 
     Differentiable in all three, once; the forward pass then keeps both
-    projections in float32. Feature counts that are not multiples of 8 cost
-    zero-padded copies of the operands.
+    projections in float32. The backward pass rounds their gradients to x's dtype
+    before the products that give the three results, each rounded once more: an
+    error about sqrt(2) times that of one rounding, and in float16 gradients of the
+    projections have float16's range (scale the loss). Feature counts that are not
+    multiples of 8 cost zero-padded copies of the operands.
     """
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, "
