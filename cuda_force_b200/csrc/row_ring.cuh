@@ -7,7 +7,7 @@
 namespace cfb {
 namespace {
 
-// The ring of one group of kTpr threads: each stage holds a row of up to
+// The ring of one group of threads: each stage holds a row of up to
 // kArrays inputs. Thread 0 of the group issues the copies; every thread waits.
 // A wait that runs out records the error and stops all later waits and copies
 // of the thread, and the kernel runs to its end on what is there.
